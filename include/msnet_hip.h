@@ -234,6 +234,28 @@ int msnet_conv3d_k3_in_f16s(const float* x_ndhwc, const void* wpk_f16s, const fl
 int msnet_conv3d_k3_cout1(const float* x, const float* w, float wscale, const float* add, float* y, int N, int D,
                           int H, int W, int Ci, msnet_stream_t stream);
 
+/* ---- group norm ------------------------------------------------------------------------------ */
+/* Group normalisation with an activation, channels-last, for aggregators normalised per sample instead of per batch:
+ *   y = act( (x - mean) / sqrt(var + eps) * weight[c] + bias[c] (+ residual) ),   mean and var over the S rows and C/G channels
+ * of one sample and group.  x, residual, y: [N][S][C] of `dtype` (0 float32, 1 float16, 2 bfloat16), S = D*H*W; channels are
+ * consecutive, rows (_ss) and samples (_sn) lie that many elements apart (a channel slice of a wider tensor, 0 for a broadcast
+ * input).  y may be x or residual itself (same strides), and must not overlap them otherwise.  act: 0 none, 1 ReLU, 2 SiLU.
+ * weight, bias: f32[C] or NULL (1 and 0).  stats: double[N][G][2], gets mean and 1 / sqrt(var + eps) for the backward; or NULL.
+ * Sums are 64-bit, in a fixed order.  float32 outputs raise bit 0 of the calling thread's overflow word as the convs' do.
+ * workspace: msnet_group_norm_workspace_bytes() bytes, 16-byte aligned (0: not needed).  N or S zero: nothing is done. */
+size_t msnet_group_norm_workspace_bytes(int dtype, int N, long S, int C, int G);
+int    msnet_group_norm(const void* x, const float* weight, const float* bias, const void* residual, void* y, double* stats,
+                        int dtype, int act, int N, long S, int C, int G, double eps, long x_sn, long x_ss, long r_sn, long r_ss,
+                        long y_sn, long y_ss, void* workspace, size_t workspace_bytes, msnet_stream_t stream);
+/* Its gradients from dy and what the forward had (stats included).  dx, dresidual: dense [N][S][C]; dweight, dbias: f32[C]; each
+ * may be NULL.  dresidual only with an activation (without one it is dy itself).  The derivative of the ReLU at 0 is 0; on which
+ * side of it a value lies is decided in 64 bits.  N or S zero: dweight and dbias become zero. */
+size_t msnet_group_norm_backward_workspace_bytes(int dtype, int N, long S, int C, int G);
+int    msnet_group_norm_backward(const void* dy, const void* x, const float* weight, const float* bias, const void* residual,
+                                 const double* stats, void* dx, void* dresidual, float* dweight, float* dbias, int dtype, int act,
+                                 int N, long S, int C, int G, long dy_sn, long dy_ss, long x_sn, long x_ss, long r_sn, long r_ss,
+                                 void* workspace, size_t workspace_bytes, msnet_stream_t stream);
+
 /* ---- tails ---------------------------------------------------------------------------------- */
 /* softmax over D + sum_d d*p_d.  gcnet_3dcnn.py:126-141.  logits f32[N][D][H][W] -> disp f32[N][H][W]. */
 int msnet_softargmin(const float* logits, float* disp, int N, int D, int H, int W, msnet_stream_t stream);
@@ -269,6 +291,17 @@ int msnet_trilinear_softargmin(const float* cost, float* disp, int N, int d, int
  * divides: epe = out3[0] / out3[2], rate = out3[1] / out3[2]).  gt, pred: f32[n]; out3: device double[3]. */
 int msnet_epe_badx(const float* gt, const float* pred, size_t n, float max_disp, float threshold, double* out3,
                    msnet_stream_t stream);
+
+/* ---- training-side: the global gradient norm and clipping -------------------------------------- */
+/* norm = sqrt(sum of the squares of all values of all `count` tensors); out = in * min(1, max_norm / (norm + 1e-6)).
+ * The four / five arrays are HOST arrays of `count` entries (device pointers, lengths, types 0 float32 / 1 float16 / 2 bfloat16);
+ * an output has its input's type or float32, and may be the input itself.  out_host = NULL: the norm alone.  norm: device f32.
+ * An infinite norm scales every finite value to 0 and a NaN makes every value one: nothing is checked on the host.  Outputs that
+ * overlap anything else of the call are refused.  workspace: msnet_clip_grads_workspace_bytes() bytes, 8-byte aligned. */
+size_t msnet_clip_grads_workspace_bytes(const int64_t* n_host, int count);
+int    msnet_clip_grads(const void* const* in_host, void* const* out_host, const int64_t* n_host, const uint8_t* in_types_host,
+                        const uint8_t* out_types_host, int count, double max_norm, float* norm, void* workspace,
+                        size_t workspace_bytes, msnet_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -78,6 +78,14 @@ SIGNATURES = {
     "msnet_deconv5_softargmin_ws": (c_int, [P, P, c_float, c_float, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P]),
     "msnet_deconv3d_cout1": (c_int, [P, P, c_float, P, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "msnet_trilinear_softargmin": (c_int, [P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),
+    "msnet_group_norm_workspace_bytes": (c_size_t, [c_int, c_int, c_long, c_int, c_int]),
+    "msnet_group_norm": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_long, c_int, c_int, ctypes.c_double, c_long, c_long, c_long, c_long,
+                                 c_long, c_long, P, c_size_t, P]),
+    "msnet_group_norm_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_long, c_int, c_int]),
+    "msnet_group_norm_backward": (c_int, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_long, c_int, c_int, c_long, c_long, c_long,
+                                          c_long, c_long, c_long, P, c_size_t, P]),
+    "msnet_clip_grads_workspace_bytes": (c_size_t, [P, c_int]),
+    "msnet_clip_grads": (c_int, [P, P, P, P, P, c_int, ctypes.c_double, P, P, c_size_t, P]),
     "msnet_epe_badx": (c_int, [P, P, c_size_t, c_float, c_float, P, P]),
 }
 

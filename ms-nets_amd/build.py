@@ -14,6 +14,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmsnet_hip.so")
 ARCH = "gfx950"
 
+# gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # (source, extra flags).  volume.hip reproduces float32 operation order => no FMA contraction there.
 SOURCES = [
     ("api.cpp", []),
@@ -31,6 +34,11 @@ SOURCES = [
     ("conv3d_f16s_wd.hip", []),
     ("tail.hip", []),
     ("metrics.hip", []),
+    ("group_norm.hip", NO_PACKED_FP32),
+    ("group_norm_backward.hip", NO_PACKED_FP32),
+    ("group_norm_backward_f16.hip", NO_PACKED_FP32),
+    ("group_norm_backward_bf16.hip", NO_PACKED_FP32),
+    ("grad_clip.hip", NO_PACKED_FP32),
     ("volume.hip", ["-ffp-contract=off"]),
     # -fno-slp-vectorize: hipcc otherwise packs the ZSAD add chains into v_pk_add_f32 + v_and (no |x| modifier) + v_mov
     ("volume_fused.hip", ["-ffp-contract=off", "-fno-slp-vectorize"]),
@@ -104,7 +112,8 @@ def build(force=False, verbose=True, defines=(), lib=None):
 
 
 def _build_locked(hipcc, objdir, out, force, verbose, defines):
-    headers = [os.path.join(CSRC, h) for h in ("common.h", "conv_common.h", "conv_f16s.h", "conv_f16s_ws.h")] + [
+    headers = [os.path.join(CSRC, h) for h in ("common.h", "conv_common.h", "conv_f16s.h", "conv_f16s_ws.h", "group_norm.h",
+                                                  "group_norm_backward.h")] + [
         os.path.join(HERE, "..", "include", "msnet_hip.h")]
     objs, procs, stamps = [], [], {}
     for src, extra in SOURCES:

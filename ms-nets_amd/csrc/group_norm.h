@@ -1,0 +1,150 @@
+// What the forward and backward kernels of the group norm share: shapes and chunks, row access, the sums over a group.
+//
+//   mean_g = (1/m) sum x,  var_g = (1/m) sum (x - mean_g)^2,  m = S * C/G values of one sample and group
+//   xhat = (x - mean) / sqrt(var + eps),   z = xhat * gamma_c + beta_c (+ residual),   y = act(z)
+//
+// Channels-last rows ([N][S][C], S = all spatial positions): one thread keeps the same V channels of a row (one vector of up to
+// 16 bytes) and walks down the rows, so its channels' constants stay in registers and a wave reads whole consecutive rows.
+#pragma once
+#include "common.h"
+
+namespace msnet {
+namespace gn {
+
+constexpr int kThreads = 256;          // of the streaming kernels; the channels of a chunk are at most kThreads * V
+enum Act { kNone = 0, kRelu = 1, kSilu = 2 };
+enum DType { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+// V values as they lie in memory.  Rows of any stride and views of any offset are taken: gfx950's global loads and stores of up to
+// 16 bytes need no more alignment than the element's own.
+template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
+template <class T> struct Pack<T, 1> { typedef T type; };
+
+template <class T, int V>
+__device__ __forceinline__ typename Pack<T, V>::type load_raw(const T* p) { return *reinterpret_cast<const typename Pack<T, V>::type*>(p); }
+
+template <class T, int V>
+__device__ __forceinline__ float element(const typename Pack<T, V>::type& r, int e) {
+    if constexpr (V == 1) return (float)r;
+    else return (float)r[e];
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+    if constexpr (V == 1) { *p = (T)f[0]; }
+    else {
+        typename Pack<T, V>::type o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = (T)f[e];
+        *reinterpret_cast<typename Pack<T, V>::type*>(p) = o;
+    }
+}
+
+struct Rows { long sn, ss; };          // elements from sample to sample and from row to row; channels are consecutive
+
+// How the channels and rows of a call are cut.  A chunk is what one workgroup's row segment covers: `gpc` whole groups (nsub = 1),
+// or, where one group is wider than a workgroup, `cw` channels of it (nsub chunks a group, gpc = 1).
+struct Shape {
+    int N, C, G, cg;                   // cg = C / G
+    long S;
+    int gpc, nsub, cw, chunks;
+    int nblk;                          // row blocks of a sample
+    long rows;                         // rows of one of them
+};
+
+struct Chunk {
+    int n, blk, g0, ng, c0, cw, sub;
+    long r0, r1;
+};
+
+__device__ __forceinline__ Chunk chunk_of(const Shape& s, unsigned b) {
+    Chunk k;
+    const unsigned chunk = b % (unsigned)s.chunks, t = b / (unsigned)s.chunks;
+    k.blk = (int)(t % (unsigned)s.nblk);
+    k.n = (int)(t / (unsigned)s.nblk);
+    if (s.nsub > 1) {
+        k.g0 = (int)chunk / s.nsub; k.sub = (int)chunk % s.nsub; k.ng = 1;
+        k.c0 = k.g0 * s.cg + k.sub * s.cw;
+        k.cw = min(s.cw, s.cg - k.sub * s.cw);
+    } else {
+        k.g0 = (int)chunk * s.gpc; k.sub = 0; k.ng = min(s.gpc, s.G - k.g0);
+        k.c0 = k.g0 * s.cg; k.cw = k.ng * s.cg;
+    }
+    k.r0 = (long)k.blk * s.rows;
+    k.r1 = min(k.r0 + s.rows, s.S);
+    return k;
+}
+
+// Adds the rows of tab[rows][cols] into row 0, pairwise and in a fixed order; every thread of the workgroup takes part.
+__device__ __forceinline__ void sum_rows(double2* tab, int rows, int cols, int tid, int threads) {
+    int p = 1;
+    while (p < rows) p <<= 1;
+    for (int step = p >> 1; step > 0; step >>= 1) {
+        __syncthreads();
+        for (int i = tid; i < step * cols; i += threads)
+            if (i + step * cols < rows * cols) tab[i] = tab[i] + tab[i + step * cols];
+    }
+    __syncthreads();
+}
+
+// f(group, sum of its `per` consecutive columns of tab, each first put through w), called by one thread a group.
+template <class W, class F>
+__device__ __forceinline__ void sum_groups(const double2* tab, int per, int ng, int tid, int threads, W w, F f) {
+    int lanes = 1;                     // threads of a group: a power of two, inside one wave
+    while (lanes < 64 && 2 * lanes <= per && 2 * lanes * ng <= threads) lanes <<= 1;
+    const int lane = tid & (lanes - 1);
+    for (int g = tid / lanes; g < ng; g += threads / lanes) {
+        double2 s = make_double2(0., 0.);
+        for (int i = lane; i < per; i += lanes) s = s + w(g * per + i, tab[g * per + i]);
+        for (int o = lanes >> 1; o > 0; o >>= 1) s = s + make_double2(__shfl_xor(s.x, o), __shfl_xor(s.y, o));
+        if (lane == 0) f(g, s);
+    }
+}
+
+// The sums of groups g0 .. g0 + ng over a sample's slots, part[slot][G]: f(group - g0, sum) by one thread a group.
+template <class F>
+__device__ __forceinline__ void sum_slots(const double2* __restrict__ part, int slots, int G, int g0, int ng, double2* tab, int tid, F f) {
+    for (int gt = 0; gt < ng; gt += kThreads) {
+        const int w = min(ng - gt, kThreads), lanes = kThreads / w;
+        const int gi = tid % w, lane = tid / w;
+        if (lane < lanes) {
+            double2 s = make_double2(0., 0.);
+            const double2* p = part + g0 + gt + gi;
+#pragma unroll 4
+            for (int i = lane; i < slots; i += lanes) s = s + p[(size_t)i * G];
+            tab[tid] = s;
+        }
+        sum_rows(tab, lanes, w, tid, kThreads);
+        if (tid < w) f(gt + tid, tab[tid]);
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ float silu_gate(float z) {       // 1 / (1 + e^-z)
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == kRelu) return z < 0.f ? 0.f : z;     // (a NaN stays one)
+    else if constexpr (ACT == kSilu) return z * silu_gate(z);
+    else return z;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+inline int element_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+// Channels a thread takes at once: 16 bytes of them where the channel count allows, 8 bytes for 16-bit types whose count is only a
+// multiple of four (C = 60: 8-byte lanes), single ones otherwise.
+inline int vector_width(int C, int dtype) {
+    const int full = 16 / element_bytes(dtype);
+    return C % full == 0 ? full : C % 4 == 0 ? 4 : 1;
+}
+
+int check_shape(const char* what, int dtype, int act, int N, long S, int C, int G, double eps);
+// V may be lowered to 1: groups whose edges fall inside vectors and that are too wide to be cut at a common multiple.
+Shape make_shape(int N, long S, int C, int G, int* V, long most_cw);
+void cut_rows(Shape* s, int V, long most_blocks, int least_passes);
+
+}  // namespace gn
+}  // namespace msnet

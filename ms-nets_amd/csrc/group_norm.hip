@@ -1,0 +1,405 @@
+// Group norm with an activation over channels-last activations, forward: y = act(xhat * gamma + beta (+ residual)).
+//
+// Two ways, by size:
+//   * group_norm_small: a chunk of whole groups of one sample fits the registers of one workgroup; it is read once, in one launch.
+//   * group_norm_stats + group_norm_apply: every row block's sums per group go to the workspace, and each workgroup of the second
+//     kernel adds up its groups' sums before it normalises; x is read twice, y written once.
+//
+// Sums are of x - pivot and its square, in 64 bits (pivot: the group's first value): no cancellation for any mean, and the sign of
+// a value next to a ReLU's border comes out as in exact arithmetic, which the backward pass relies on.  gfx950 adds doubles at the
+// rate of floats, so the sums cost no more than three instructions a value.
+#include "group_norm.h"
+
+namespace msnet {
+namespace gn {
+
+int check_shape(const char* what, int dtype, int act, int N, long S, int C, int G, double eps) {
+    if (dtype < kF32 || dtype > kBF16) return fail("%s: dtype %d is none of 0 (float32), 1 (float16), 2 (bfloat16)", what, dtype);
+    if (act < kNone || act > kSilu) return fail("%s: activation %d is none of 0 (none), 1 (ReLU), 2 (SiLU)", what, act);
+    if (N < 0 || S < 0 || C <= 0) return fail("%s: bad shape N=%d S=%ld C=%d", what, N, S, C);
+    if (G <= 0 || C % G != 0) return fail("%s: %d groups do not divide %d channels", what, G, C);
+    if (!(eps >= 0.)) return fail("%s: eps=%g", what, eps);
+    return 0;
+}
+
+static int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+Shape make_shape(int N, long S, int C, int G, int* V, long most_cw) {
+    Shape s = {};
+    s.N = N; s.S = S; s.C = C; s.G = G; s.cg = C / G;
+    int step = *V / gcd(s.cg, *V);                         // groups between two edges that are edges of vectors too
+    if (step > 1 && (long)s.cg * step > (long)kThreads * *V) { *V = 1; step = 1; }
+    const long widest = (long)kThreads * *V;
+    if ((long)s.cg * step > widest) {
+        s.gpc = 1; s.cw = (int)widest; s.nsub = (int)((s.cg + widest - 1) / widest); s.chunks = G * s.nsub;
+    } else {
+        const long w = most_cw < widest ? most_cw : widest, unit = (long)s.cg * step;
+        const int most = (int)(w / unit > 0 ? w / unit : 1) * step;
+        s.chunks = (G + most - 1) / most;
+        s.gpc = ((G + s.chunks - 1) / s.chunks + step - 1) / step * step;
+        s.chunks = (G + s.gpc - 1) / s.gpc;
+        s.nsub = 1; s.cw = (s.gpc < G ? s.gpc : G) * s.cg;
+    }
+    s.nblk = 1; s.rows = S;
+    return s;
+}
+
+void cut_rows(Shape* s, int V, long most_blocks, int least_passes) {
+    const long per_pass = kThreads / (s->cw / V), least = per_pass * least_passes;
+    long nblk = most_blocks / ((long)s->N * s->chunks);
+    if (nblk > (s->S + least - 1) / least) nblk = (s->S + least - 1) / least;
+    if (nblk < 1) nblk = 1;
+    s->rows = ((s->S + nblk - 1) / nblk + per_pass - 1) / per_pass * per_pass;
+    s->nblk = (int)((s->S + s->rows - 1) / s->rows);
+}
+
+// mean and 1 / sqrt(var + eps) from the sums of x - pivot and of its square over m values
+__device__ __forceinline__ double2 statistics(double2 sum, double pivot, double m, double eps) {
+    const double d = sum.x / m;
+    double var = sum.y / m - d * d;
+    var = var < 0. ? 0. : var;
+    return make_double2(pivot + d, 1. / sqrt(var + eps));
+}
+
+// What a thread keeps of its channels: z = (x - mean) * scale + shift with the mean's own rounding folded into shift.
+template <int V>
+struct Affine {
+    float mean[V], scale[V], shift[V];
+    __device__ __forceinline__ void set(const double2* st, int c_local, int c, int cg, const float* weight, const float* bias) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double2 t = st[(c_local + e) / cg];
+            const double a = weight ? t.y * (double)weight[c + e] : t.y;
+            mean[e] = (float)t.x;
+            scale[e] = (float)a;
+            shift[e] = (float)((bias ? (double)bias[c + e] : 0.) - (t.x - (double)mean[e]) * a);
+        }
+    }
+};
+
+// One row's V values: normalise, add the residual, activate, store; amax gathers magnitude bits for the range guard.
+template <class T, int V, int ACT>
+__device__ __forceinline__ void finish(const Affine<V>& k, const typename Pack<T, V>::type& x, const typename Pack<T, V>::type& res, bool has_res,
+                                       T* y, bool guard, unsigned& amax) {
+    float o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        float z = fmaf(element<T, V>(x, e) - k.mean[e], k.scale[e], k.shift[e]);
+        if (has_res) z += element<T, V>(res, e);
+        o[e] = activate<ACT>(z);
+    }
+    if (guard)
+#pragma unroll
+        for (int e = 0; e < V; ++e) amax = max(amax, __builtin_bit_cast(unsigned, o[e]) & 0x7fffffffu);
+    store<T, V>(y, o);
+}
+
+// Per-thread sums into the workgroup's table: one column a vector where a vector lies in one group, one a channel elsewhere.
+template <int V>
+__device__ __forceinline__ void put_sums(double2* tab, int tid, bool whole, const double (&s)[V], const double (&q)[V]) {
+    if (whole) {
+        double a = s[0], b = q[0];
+#pragma unroll
+        for (int e = 1; e < V; ++e) { a += s[e]; b += q[e]; }
+        tab[tid] = make_double2(a, b);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) tab[tid * V + e] = make_double2(s[e], q[e]);
+    }
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict__ x, Rows xr, Shape sh, double2* __restrict__ part,
+                                                             double* __restrict__ pivots) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];
+    const Chunk k = chunk_of(sh, blockIdx.x);
+    const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V;
+    const bool whole = sh.cg % V == 0;
+    const T* xn = x + (size_t)k.n * xr.sn;
+    double pivot[V], s[V], q[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        pivot[e] = (double)(float)xn[(size_t)(k.g0 + (k.ng > 1 ? (cl + e) / sh.cg : 0)) * sh.cg];
+        s[e] = q[e] = 0.;
+    }
+    if (k.blk == 0 && k.sub == 0)
+        for (int g = tid; g < k.ng; g += kThreads) pivots[(size_t)k.n * sh.G + k.g0 + g] = (double)(float)xn[(size_t)(k.g0 + g) * sh.cg];
+    if (row < per_pass) {
+        const T* p = xn + k.c0 + cl;
+        long r = k.r0 + row;
+        auto add = [&](const typename Pack<T, V>::type& v) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const double d = (double)element<T, V>(v, e) - pivot[e];
+                s[e] += d;
+                q[e] = fma(d, d, q[e]);
+            }
+        };
+        for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {       // four loads in flight a thread
+            typename Pack<T, V>::type v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = load_raw<T, V>(p + (size_t)(r + (long)u * per_pass) * xr.ss);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) add(v[u]);
+        }
+        for (; r < k.r1; r += per_pass) add(load_raw<T, V>(p + (size_t)r * xr.ss));
+        put_sums<V>(tab, tid, whole, s, q);
+    }
+    const int cols = whole ? cv : k.cw;
+    sum_rows(tab, per_pass, cols, tid, kThreads);
+    const size_t slot = (size_t)k.n * sh.nblk * sh.nsub + (size_t)k.blk * sh.nsub + k.sub;
+    sum_groups(tab, cols / k.ng, k.ng, tid, kThreads, [](int, double2 v) { return v; },
+               [&](int g, double2 v) { part[slot * sh.G + k.g0 + g] = v; });
+}
+
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr, const float* __restrict__ weight,
+                                                             const float* __restrict__ bias, const T* residual, Rows rr, T* y, Rows yr,
+                                                             double2* __restrict__ stats, Shape sh, int slots,
+                                                             const double2* __restrict__ part, const double* __restrict__ pivots,
+                                                             double m, double eps, unsigned* oflag) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics
+    double2* st = tab + kThreads;
+    // last rows first: what the sums read last is what the caches still hold
+    const Chunk k = chunk_of(sh, gridDim.x - 1 - blockIdx.x);
+    const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V;
+    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid, [&](int g, double2 sum) {
+        const size_t at = (size_t)k.n * sh.G + k.g0 + g;
+        const double2 t = statistics(sum, pivots[at], m, eps);
+        st[g] = t;
+        if (stats && k.blk == 0 && k.sub == 0) stats[at] = t;
+    });
+    if (row >= per_pass) return;
+    Affine<V> a;
+    a.set(st, cl, k.c0 + cl, k.ng > 1 ? sh.cg : k.cw, weight, bias);
+    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
+    const T* pr = residual ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
+    const long rs = residual ? rr.ss : xr.ss;
+    T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
+    unsigned amax = 0u;
+    long r = k.r0 + row;
+    for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {
+        typename Pack<T, V>::type v[4], w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+        if (residual)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+        else
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = v[u];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, oflag != nullptr, amax);
+    }
+    for (; r < k.r1; r += per_pass) {
+        const auto v = load_raw<T, V>(px + (size_t)r * xr.ss);
+        const auto w = load_raw<T, V>(pr + (size_t)r * rs);
+        finish<T, V, ACT>(a, v, w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
+    }
+    if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);            // |y| >= 32752, inf or NaN: as the convs' epilogues
+}
+
+// M: vectors a thread holds.  A workgroup takes all rows of one chunk of one sample.
+template <class T, int V, int M, int ACT>
+__global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, const float* __restrict__ weight, const float* __restrict__ bias,
+                                                         const T* residual, Rows rr, T* y, Rows yr, double2* __restrict__ stats, Shape sh,
+                                                         double m, double eps, unsigned* oflag) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];
+    const Chunk k = chunk_of(sh, blockIdx.x);
+    const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V;
+    const bool whole = sh.cg % V == 0;
+    const int cols = whole ? cv : k.cw;
+    double2* st = tab + (whole ? threads : threads * V);
+    const T* xn = x + (size_t)k.n * xr.sn;
+    const T* px = xn + k.c0 + cl;
+    const int S = (int)sh.S;
+    typename Pack<T, V>::type v[M];
+    if (row < per_pass) {
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (row + i * per_pass < S) v[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
+    }
+    double pivot[V], s[V], q[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        pivot[e] = (double)(float)xn[(size_t)(k.g0 + (cl + e) / sh.cg) * sh.cg];
+        s[e] = q[e] = 0.;
+    }
+    if (row < per_pass) {
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (row + i * per_pass < S)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const double d = (double)element<T, V>(v[i], e) - pivot[e];
+                    s[e] += d;
+                    q[e] = fma(d, d, q[e]);
+                }
+        put_sums<V>(tab, tid, whole, s, q);
+    }
+    sum_rows(tab, per_pass, cols, tid, threads);
+    sum_groups(tab, cols / k.ng, k.ng, tid, threads, [](int, double2 u) { return u; }, [&](int g, double2 sum) {
+        const double2 t = statistics(sum, (double)(float)xn[(size_t)(k.g0 + g) * sh.cg], m, eps);
+        st[g] = t;
+        if (stats) stats[(size_t)k.n * sh.G + k.g0 + g] = t;
+    });
+    __syncthreads();                                       // statistics are there, and nobody reads x any more (y may be x)
+    if (row >= per_pass) return;
+    Affine<V> a;
+    a.set(st, cl, k.c0 + cl, sh.cg, weight, bias);
+    const T* pr = residual ? residual + (size_t)k.n * rr.sn + k.c0 + cl : nullptr;
+    T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
+    unsigned amax = 0u;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        const int r = row + i * per_pass;
+        if (r < S) {
+            auto w = v[i];
+            if (residual) w = load_raw<T, V>(pr + (size_t)r * rr.ss);
+            finish<T, V, ACT>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
+        }
+    }
+    if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+
+struct Forward {
+    const void *x, *residual;
+    const float *weight, *bias;
+    void* y;
+    double2* stats;
+    Rows xr, rr, yr;
+    double eps;
+    unsigned* oflag;
+    hipStream_t stream;
+};
+
+constexpr long kStatsBlocks = 512, kApplyBlocks = 2048;
+
+// One workgroup a chunk: threads and vectors a thread, or 0 where the chunk does not fit.
+static int small_threads(const Shape& s, int V, int* M) {
+    const int cv = s.cw / V, most = s.cg % V == 0 ? 1024 : 2048 / V;      // (table of sums and statistics: 64 KB at most)
+    for (int m : {4, 16})
+        for (int t = 256; t <= most; t <<= 1)
+            if (s.S <= (long)m * (t / cv)) { *M = m; return t; }
+    return 0;
+}
+
+// Chunks of 64 bytes a row (half a cache line) give the single launch the most workgroups; wider ones once those fill the device.
+static Shape small_shape(int N, long S, int C, int G, int* V, int dtype) {
+    long w = 64 / element_bytes(dtype);
+    Shape s = make_shape(N, S, C, G, V, w);
+    while ((long)N * s.chunks > 2048 && w < (long)kThreads * *V) {
+        w *= 2;
+        const Shape t = make_shape(N, S, C, G, V, w);
+        int M;
+        if (t.nsub > 1 || !small_threads(t, *V, &M)) break;
+        s = t;
+    }
+    return s;
+}
+
+static size_t stats_bytes(const Shape& s) { return (size_t)s.N * s.nblk * s.nsub * s.G * sizeof(double2) + (size_t)s.N * s.G * sizeof(double); }
+
+struct Plan {
+    Shape shape;                        // of the sums, or of the one launch
+    int V, M, threads;                  // threads > 0: the single launch
+    size_t bytes;
+};
+
+static Plan plan_forward(int N, long S, int C, int G, int dtype) {
+    Plan p = {};
+    p.V = vector_width(C, dtype);
+    p.shape = small_shape(N, S, C, G, &p.V, dtype);
+    p.threads = p.shape.nsub > 1 ? 0 : small_threads(p.shape, p.V, &p.M);
+    if (!p.threads) {
+        p.V = vector_width(C, dtype);
+        p.shape = make_shape(N, S, C, G, &p.V, 1l << 40);
+        cut_rows(&p.shape, p.V, kStatsBlocks, 8);
+        p.bytes = stats_bytes(p.shape);
+    }
+    return p;
+}
+
+template <class T, int V, int ACT>
+static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) {
+    const Shape& sh = p.shape;
+    const double m = (double)sh.S * sh.cg;
+    const T *x = (const T*)f.x, *res = (const T*)f.residual;
+    const long grid = (long)sh.N * sh.nblk * sh.chunks;
+    const size_t per_table = (sh.cg % V == 0 ? 1 : V) * sizeof(double2);
+    if (p.threads) {
+        const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
+        LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
+        if (p.M == 4)
+            hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias, res,
+                               f.rr, (T*)f.y, f.yr, f.stats, sh, m, f.eps, f.oflag);
+        else
+            hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias, res,
+                               f.rr, (T*)f.y, f.yr, f.stats, sh, m, f.eps, f.oflag);
+        return check_launch("msnet_group_norm");
+    }
+    double2* part = (double2*)ws;
+    double* pivots = (double*)(part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G);
+    {
+        LaunchScope ls("group_norm_stats", f.stream, 4.0 * sh.N * m * sh.G, (double)sh.N * m * sh.G * sizeof(T));
+        hipLaunchKernelGGL((group_norm_stats<T, V>), dim3((unsigned)grid), dim3(kThreads), kThreads * per_table, f.stream, x, f.xr, sh, part, pivots);
+        if (int rc = check_launch("msnet_group_norm")) return rc;
+    }
+    Shape out = sh;
+    cut_rows(&out, V, kApplyBlocks, 4);
+    const long grid2 = (long)out.N * out.nblk * out.chunks;
+    LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
+    hipLaunchKernelGGL((group_norm_apply<T, V, ACT>), dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr,
+                       f.weight, f.bias, res, f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, m, f.eps, f.oflag);
+    return check_launch("msnet_group_norm");
+}
+
+template <class T, int V>
+static int forward_v(const Forward& f, const Plan& p, int act, void* ws, double bytes) {
+    return act == kRelu ? forward_act<T, V, kRelu>(f, p, ws, bytes) : act == kSilu ? forward_act<T, V, kSilu>(f, p, ws, bytes)
+                                                                                   : forward_act<T, V, kNone>(f, p, ws, bytes);
+}
+
+template <class T>
+static int forward_t(const Forward& f, const Plan& p, int act, void* ws, double bytes) {
+    if constexpr (sizeof(T) == 2)
+        if (p.V == 8) return forward_v<T, 8>(f, p, act, ws, bytes);
+    return p.V == 4 ? forward_v<T, 4>(f, p, act, ws, bytes) : forward_v<T, 1>(f, p, act, ws, bytes);
+}
+
+}  // namespace gn
+}  // namespace msnet
+
+using namespace msnet;
+
+extern "C" size_t msnet_group_norm_workspace_bytes(int dtype, int N, long S, int C, int G) {
+    if (gn::check_shape("msnet_group_norm_workspace_bytes", dtype, 0, N, S, C, G, 0.) || N == 0 || S == 0) return 0;
+    return gn::plan_forward(N, S, C, G, dtype).bytes;
+}
+
+extern "C" int msnet_group_norm(const void* x, const float* weight, const float* bias, const void* residual, void* y, double* stats, int dtype,
+                                int act, int N, long S, int C, int G, double eps, long x_sn, long x_ss, long r_sn, long r_ss, long y_sn, long y_ss,
+                                void* workspace, size_t workspace_bytes, msnet_stream_t stream) {
+    if (int rc = gn::check_shape("msnet_group_norm", dtype, act, N, S, C, G, eps)) return rc;
+    if (N == 0 || S == 0) return 0;
+    if (!x || !y) return fail("msnet_group_norm: null pointer");
+    if (x_sn < 0 || x_ss < 0 || r_sn < 0 || r_ss < 0 || y_sn < 0 || y_ss < 0) return fail("msnet_group_norm: negative stride");
+    if (((uintptr_t)stats | (uintptr_t)workspace) & 15) return fail("msnet_group_norm: stats and workspace must be 16-byte aligned");
+    const gn::Plan p = gn::plan_forward(N, S, C, G, dtype);
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+        return fail("msnet_group_norm: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, p.bytes);
+    // (a launch has at most 2^32 - 1 threads; row blocks are added only up to a few thousand workgroups in all)
+    if (((double)N * p.shape.chunks + 4096) * (p.threads ? p.threads : gn::kThreads) > 4294967295.)
+        return fail("msnet_group_norm: N=%d samples of %d channel chunks are too many for one launch", N, p.shape.chunks);
+    const gn::Forward f = {x, residual, weight, bias, y, (double2*)stats, {x_sn, x_ss}, {r_sn, r_ss}, {y_sn, y_ss}, eps,
+                           dtype == gn::kF32 ? overflow_flag() : nullptr, (hipStream_t)stream};
+    const double bytes = (double)N * S * C * gn::element_bytes(dtype) * (residual ? 3 : 2);
+    return dtype == gn::kF32 ? gn::forward_t<float>(f, p, act, workspace, bytes) : dtype == gn::kF16 ? gn::forward_t<_Float16>(f, p, act, workspace, bytes)
+                                                                                                    : gn::forward_t<__bf16>(f, p, act, workspace, bytes);
+}

@@ -1,0 +1,399 @@
+// Group norm with an activation, backward.  With dz = dy * act'(z), gz = gamma * dz and sums over the m values of a group:
+//
+//   dbeta_c = sum dz,   dgamma_c = sum dz * xhat          (over samples and rows)
+//   c1 = (1/m) sum gz,  c2 = (1/m) sum gz * xhat
+//   dx = (gz - c1 - xhat * c2) / sqrt(var + eps),   dresidual = dz
+//
+// xhat and z are computed again from x (and the residual) and the saved statistics; nothing but those is kept from the forward.
+// As in the forward there are two ways: group_norm_grad_small holds a chunk of one sample in registers and reads x and dy once;
+// group_norm_grad_sums leaves every row block's sums per channel and per group in the workspace and group_norm_grad_apply adds
+// them up, its first workgroups for dgamma and dbeta.  Sums are 64-bit and added in a fixed order: a result repeats bit for bit.
+//
+// A ReLU's derivative jumps at z = 0.  z in 32 bits is off by at most 2^-22 (|beta + residual| + |what the mean's rounding left|)
+// there; a vector with a value within four times that is decided in 64 bits (a few of a million are).
+#pragma once
+#include "group_norm.h"
+
+namespace msnet {
+namespace gn {
+
+struct Backward {
+    const void *dy, *x, *residual;
+    const float *weight, *bias;
+    const double2* stats;              // [N][G] mean, 1 / sqrt(var + eps)
+    void *dx, *dresidual;
+    float *dweight, *dbias;
+    Rows yr, xr, rr;                   // of dy, x, residual; dx and dresidual are dense
+    hipStream_t stream;
+};
+
+struct BackwardPlan {
+    Shape shape;
+    int V, M, threads;                 // threads > 0: the single launch
+    size_t bytes;
+};
+
+BackwardPlan plan_backward(int N, long S, int C, int G, int dtype);
+int backward_f32(const Backward& f, const BackwardPlan& p, int act, void* ws);
+int backward_f16(const Backward& f, const BackwardPlan& p, int act, void* ws);
+int backward_bf16(const Backward& f, const BackwardPlan& p, int act, void* ws);
+
+// vectors of x and dy a thread of the single launch holds (1024 threads leave 128 registers each)
+constexpr int kGradFew = 2;
+constexpr int grad_many(int V) { return V == 8 ? 4 : 8; }
+constexpr int kParamCols = 16;         // channels of one workgroup that sums dgamma and dbeta
+constexpr long kGradSumBlocks = 512, kGradApplyBlocks = 2048;
+
+// What a thread keeps of its V channels.
+template <int V>
+struct Channels {
+    float mean[V], rstd[V], lo[V], gamma[V], beta[V], near[V];
+    __device__ __forceinline__ void set(const double2* st, int c_local, int c, int cg, const float* weight, const float* bias) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double2 t = st[(c_local + e) / cg];
+            mean[e] = (float)t.x;
+            rstd[e] = (float)t.y;
+            lo[e] = (float)(((double)mean[e] - t.x) * t.y);
+            gamma[e] = weight ? weight[c + e] : 1.f;
+            beta[e] = bias ? bias[c + e] : 0.f;
+            near[e] = gamma[e] == 0.f ? -1.f : 0x1p-20f * fabsf(lo[e] * gamma[e]);       // (gamma = 0: z is exact)
+        }
+    }
+};
+
+// dz and xhat of one row's V values.
+template <class T, int V, int ACT, bool RES>
+__device__ __forceinline__ void derive(const Channels<V>& k, const double2* st, int c_local, int cg, const typename Pack<T, V>::type& x,
+                                       const typename Pack<T, V>::type& dy, const typename Pack<T, V>::type& res, float (&dz)[V], float (&xhat)[V]) {
+    float z[V];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        xhat[e] = fmaf(element<T, V>(x, e) - k.mean[e], k.rstd[e], k.lo[e]);
+        if constexpr (ACT != kNone) {
+            const float b = RES ? k.beta[e] + element<T, V>(res, e) : k.beta[e];
+            z[e] = fmaf(xhat[e], k.gamma[e], b);
+            if constexpr (ACT == kRelu) near |= fabsf(z[e]) <= fmaf(fabsf(b), 0x1p-20f, k.near[e]);
+        }
+    }
+    if constexpr (ACT == kRelu)
+        if (near)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                int c = c_local + e;                       // opaque to the compiler: it would form these doubles outside the loop over
+                float g = k.gamma[e], b = k.beta[e];       // the rows, for every thread, and spill registers to keep them
+                asm volatile("" : "+v"(c), "+v"(g), "+v"(b));
+                const double2 t = st[c / cg];
+                double d = ((double)element<T, V>(x, e) - t.x) * t.y * (double)g + (double)b;
+                if constexpr (RES) d += (double)element<T, V>(res, e);
+                z[e] = d > 0. ? 1.f : 0.f;
+            }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float g = element<T, V>(dy, e);
+        if constexpr (ACT == kRelu) dz[e] = z[e] > 0.f ? g : 0.f;
+        else if constexpr (ACT == kSilu) {
+            const float sig = silu_gate(z[e]);
+            dz[e] = g * (sig * fmaf(z[e], 1.f - sig, 1.f));
+        } else dz[e] = g;
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void grad_input(const Channels<V>& k, const float (&c1)[V], const float (&c2)[V], const float (&dz)[V],
+                                           const float (&xhat)[V], float (&dx)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float gz = k.gamma[e] * dz[e];       // (rounded before the subtraction: a group of one value has gz = c1 and dx = 0)
+        dx[e] = (__fsub_rn(gz, c1[e]) - xhat[e] * c2[e]) * k.rstd[e];
+    }
+}
+
+// dgamma and dbeta of kParamCols channels from chan[rows][C].
+__device__ __forceinline__ void param_grads(const double2* __restrict__ chan, long rows, int C, int block, float* dweight, float* dbias, double2* tab) {
+    const int tid = threadIdx.x, col = tid % kParamCols, lane = tid / kParamCols, c = block * kParamCols + col;
+    double2 s = make_double2(0., 0.);
+    if (c < C)
+#pragma unroll 4
+        for (long i = lane; i < rows; i += kThreads / kParamCols) s = s + chan[(size_t)i * C + c];
+    tab[tid] = s;
+    sum_rows(tab, kThreads / kParamCols, kParamCols, tid, kThreads);
+    if (tid < kParamCols && c < C) {
+        if (dbias) dbias[c] = (float)tab[tid].x;
+        if (dweight) dweight[c] = (float)tab[tid].y;
+    }
+}
+
+template <int UNUSED>
+__global__ __launch_bounds__(kThreads) void group_norm_param_grads(const double2* __restrict__ chan, long rows, int C, float* dweight, float* dbias) {
+    __shared__ double2 tab[kThreads];
+    param_grads(chan, rows, C, blockIdx.x, dweight, dbias, tab);
+}
+
+template <class T, int V, int ACT, bool RES>
+__global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
+                                                                 const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
+                                                                 const float* __restrict__ bias, const double2* __restrict__ stats, Shape sh,
+                                                                 double2* __restrict__ part, double2* __restrict__ chan) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads * V] sums, [ng] statistics
+    double2* st = tab + kThreads * V;
+    const Chunk k = chunk_of(sh, blockIdx.x);
+    const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
+    for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
+    __syncthreads();
+    if (row < per_pass) {
+        Channels<V> a;
+        a.set(st, cl, k.c0 + cl, cg, weight, bias);
+        double s[V], q[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
+        const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
+        const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
+        const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
+        const long rs = RES ? rr.ss : xr.ss;
+        auto add = [&](const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
+            float dz[V], xhat[V];
+            derive<T, V, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s[e] += (double)dz[e];
+                q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
+            }
+        };
+        long r = k.r0 + row;
+        for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {
+            typename Pack<T, V>::type vx[4], vd[4], vr[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
+                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+                else vr[u] = vx[u];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) add(vx[u], vd[u], vr[u]);
+        }
+        for (; r < k.r1; r += per_pass)
+            add(load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+#pragma unroll
+        for (int e = 0; e < V; ++e) tab[tid * V + e] = make_double2(s[e], q[e]);
+    }
+    sum_rows(tab, per_pass, k.cw, tid, kThreads);
+    double2* mine = chan + ((size_t)k.n * sh.nblk + k.blk) * sh.C + k.c0;
+    for (int c = tid; c < k.cw; c += kThreads) mine[c] = tab[c];
+    const size_t slot = (size_t)k.n * sh.nblk * sh.nsub + (size_t)k.blk * sh.nsub + k.sub;
+    sum_groups(tab, k.cw / k.ng, k.ng, tid, kThreads,
+               [&](int c, double2 v) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * v.x, g * v.y); },
+               [&](int g, double2 v) { part[slot * sh.G + k.g0 + g] = v; });
+}
+
+template <class T, int V, int ACT, bool RES>
+__global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
+                                                                  const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
+                                                                  const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
+                                                                  T* __restrict__ dresidual, float* dweight, float* dbias, Shape sh, int slots,
+                                                                  const double2* __restrict__ part, const double2* __restrict__ chan, long chan_rows,
+                                                                  int param_blocks, double m) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics, [ng] c1 and c2
+    if ((int)blockIdx.x < param_blocks) {
+        param_grads(chan, chan_rows, sh.C, blockIdx.x, dweight, dbias, tab);
+        return;
+    }
+    const Chunk k = chunk_of(sh, gridDim.x - 1 - blockIdx.x);          // last rows first, as in the forward
+    double2 *st = tab + kThreads, *coef = st + k.ng;
+    const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
+    for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
+    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid,
+              [&](int g, double2 sum) { coef[g] = make_double2(sum.x / m, sum.y / m); });
+    if (row >= per_pass) return;
+    Channels<V> a;
+    a.set(st, cl, k.c0 + cl, cg, weight, bias);
+    float c1[V], c2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
+    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
+    const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
+    const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
+    const long rs = RES ? rr.ss : xr.ss;
+    const size_t dense = (size_t)k.n * sh.S * sh.C + k.c0 + cl;
+    auto one = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
+        float dz[V], xhat[V], o[V];
+        derive<T, V, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
+        grad_input<V>(a, c1, c2, dz, xhat, o);
+        if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
+        if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
+    };
+    long r = k.r0 + row;
+    for (; r + per_pass < k.r1; r += 2l * per_pass) {
+        typename Pack<T, V>::type vx[2], vd[2], vr[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+            vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
+            if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+            else vr[u] = vx[u];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) one(r + (long)u * per_pass, vx[u], vd[u], vr[u]);
+    }
+    if (r < k.r1) one(r, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+}
+
+// All rows of one chunk of one sample in registers, M vectors of x and of dy a thread.  direct: one sample, its channel sums are
+// dgamma and dbeta; else they go to chan[N][C].
+template <class T, int V, int M, int ACT, bool RES>
+__global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
+                                                              const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
+                                                              const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
+                                                              T* __restrict__ dresidual, float* dweight, float* dbias, Shape sh,
+                                                              double2* __restrict__ chan, bool direct, double m) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [2048] sums of a round, [cw] of the channels, [ng] statistics
+    const Chunk k = chunk_of(sh, blockIdx.x);
+    double2 *sums = tab + 2048, *st = sums + k.cw, *coef = tab;
+    const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
+    const int row = tid / cv, cl = (tid % cv) * V, cg = sh.cg;
+    const int S = (int)sh.S;
+    for (int g = tid; g < k.ng; g += threads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
+    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
+    const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
+    const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
+    typename Pack<T, V>::type vx[M], vd[M], vr[M];
+    const bool on = row < per_pass;
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (row + i * per_pass < S) {
+                vx[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
+                vd[i] = load_raw<T, V>(pd + (size_t)(row + i * per_pass) * yr.ss);
+                if constexpr (RES) vr[i] = load_raw<T, V>(pr + (size_t)(row + i * per_pass) * rr.ss);
+                else vr[i] = vx[i];
+            }
+    }
+    __syncthreads();
+    Channels<V> a;
+    double s[V], q[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
+    if (on) {
+        a.set(st, cl, k.c0 + cl, cg, weight, bias);
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+            if (row + i * per_pass < S) {
+                float dz[V], xhat[V];
+                derive<T, V, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    s[e] += (double)dz[e];
+                    q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
+                }
+            }
+    }
+    // channel sums, at most 2048 of the threads' values in the table at a time
+    const int round = min(V, 2048 / threads);
+#pragma unroll
+    for (int e0 = 0; e0 < V; ++e0) {
+        if (e0 % round) continue;
+        if (on) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e >= e0 && e < e0 + round) tab[(row * cv + cl / V) * round + e - e0] = make_double2(s[e], q[e]);
+        }
+        sum_rows(tab, per_pass, cv * round, tid, threads);
+        for (int i = tid; i < cv * round; i += threads) sums[i / round * V + e0 + i % round] = tab[i];
+        __syncthreads();
+    }
+    for (int c = tid; c < k.cw; c += threads) {
+        if (direct) {
+            if (dbias) dbias[k.c0 + c] = (float)sums[c].x;
+            if (dweight) dweight[k.c0 + c] = (float)sums[c].y;
+        } else if (chan) chan[(size_t)k.n * sh.C + k.c0 + c] = sums[c];
+    }
+    sum_groups(sums, cg, k.ng, tid, threads,
+               [&](int c, double2 v) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * v.x, g * v.y); },
+               [&](int g, double2 v) { coef[g] = make_double2(v.x / m, v.y / m); });
+    __syncthreads();
+    if (!on) return;
+    float c1[V], c2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
+    const size_t dense = (size_t)k.n * sh.S * sh.C + k.c0 + cl;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        const int r = row + i * per_pass;
+        if (r < S) {
+            float dz[V], xhat[V], o[V];
+            derive<T, V, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+            grad_input<V>(a, c1, c2, dz, xhat, o);
+            if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
+            if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+
+template <class T, int V, int ACT, bool RES>
+static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
+    const Shape& sh = p.shape;
+    const double m = (double)sh.S * sh.cg, values = m * sh.N * sh.G;
+    const T *dy = (const T*)f.dy, *x = (const T*)f.x, *res = (const T*)f.residual;
+    T *dx = (T*)f.dx, *dres = (T*)f.dresidual;
+    const bool params = f.dweight || f.dbias;
+    const unsigned param_blocks = params ? (unsigned)((sh.C + kParamCols - 1) / kParamCols) : 0;
+    const unsigned grid = (unsigned)((long)sh.N * sh.nblk * sh.chunks);
+    if (p.threads) {
+        const bool direct = sh.N == 1;
+        double2* chan = direct || !params ? nullptr : (double2*)ws;
+        const size_t lds = (2048 + sh.cw + sh.gpc) * sizeof(double2);
+        {
+            LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
+            if (p.M == kGradFew)
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
+            else
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, grad_many(V), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
+            if (int rc = check_launch("msnet_group_norm_backward")) return rc;
+        }
+        if (!chan) return 0;
+        LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.C);
+        hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N, sh.C, f.dweight, f.dbias);
+        return check_launch("msnet_group_norm_backward");
+    }
+    double2* part = (double2*)ws;
+    double2* chan = part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G;
+    {
+        LaunchScope ls("group_norm_grad_sums", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 3 : 2));
+        hipLaunchKernelGGL((group_norm_grad_sums<T, V, ACT, RES>), dim3(grid), dim3(kThreads), (kThreads * V + sh.gpc) * sizeof(double2), f.stream, dy,
+                           f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, sh, part, chan);
+        if (int rc = check_launch("msnet_group_norm_backward")) return rc;
+    }
+    Shape out = sh;
+    cut_rows(&out, V, kGradApplyBlocks, 4);
+    const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
+    LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
+    hipLaunchKernelGGL((group_norm_grad_apply<T, V, ACT, RES>), dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy,
+                       f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, out, sh.nblk * sh.nsub, part, chan,
+                       (long)sh.N * sh.nblk, (int)param_blocks, m);
+    return check_launch("msnet_group_norm_backward");
+}
+
+template <class T, int V>
+static int backward_v(const Backward& f, const BackwardPlan& p, int act, void* ws) {
+    if (act == kRelu) return f.residual ? backward_act<T, V, kRelu, true>(f, p, ws) : backward_act<T, V, kRelu, false>(f, p, ws);
+    if (act == kSilu) return f.residual ? backward_act<T, V, kSilu, true>(f, p, ws) : backward_act<T, V, kSilu, false>(f, p, ws);
+    return backward_act<T, V, kNone, false>(f, p, ws);        // the residual's gradient is dy itself
+}
+
+template <class T>
+static int backward_t(const Backward& f, const BackwardPlan& p, int act, void* ws) {
+    if constexpr (sizeof(T) == 2)
+        if (p.V == 8) return backward_v<T, 8>(f, p, act, ws);
+    return p.V == 4 ? backward_v<T, 4>(f, p, act, ws) : backward_v<T, 1>(f, p, act, ws);
+}
+
+}  // namespace gn
+}  // namespace msnet

@@ -6,6 +6,7 @@ file decoding (cv2.imread) and dataset lists stay with the caller.
   crop_disparity      main_msnet.py:585-589
   save_pfm / read_pfm src/utils/pfmutil.py:86-110 / :48-83   (same bytes: header 'Pf', 'W H', signed scale, rows bottom-up)
   get_epe_rate        main_msnet.py:708-713      (NumPy inputs: host; GPU tensors: csrc/metrics.hip)
+  clip_grad_norm_     the training loop's gradient clipping, on the device (csrc/grad_clip.hip; not in the reference)
   strip_module_prefix keys saved from nn.DataParallel carry 'module.' (main_msnet.py:174, 509-526)
 """
 import re
@@ -99,6 +100,19 @@ def get_epe_rate_gpu(disp, prediction, max_disp=192, threshold=3.0):
     if valid == 0:
         return float("nan"), float("nan")              # np.mean of an empty selection, as the reference would produce
     return s / valid, bad / valid
+
+
+def clip_grad_norm_(parameters, max_norm):
+    """torch.nn.utils.clip_grad_norm_ for a training loop around these kernels: scales the gradients of `parameters` (an iterable, or
+    one tensor; those without a gradient are skipped) in place to a global 2-norm of at most max_norm and returns the norm before
+    as a float32 scalar on the device.  Two launches for the whole model, and no host synchronisation (hipops.clip_grads)."""
+    import torch
+    from . import hipops
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)                            # as torch's: nothing says which device
+    return hipops.clip_grads(grads, max_norm)
 
 
 def strip_module_prefix(state_dict):

@@ -443,6 +443,282 @@ def trilinear_softargmin(cost, out_dhw):
     return disp
 
 
+# ---- group norm ------------------------------------------------------------------------------------------------------------
+
+_DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ACT_CODES = {"none": 0, "relu": 1, "silu": 2}
+
+
+def _require_gpu(t, name):
+    """A tensor of a type the training-side kernels take, on the current device (as _lib.require_gpu_f32, any layout)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if t.layout != torch.strided:
+        raise TypeError("%s must be a dense tensor (got %s)" % (name, t.layout))
+    if not t.is_cuda:
+        raise RuntimeError("%s must live on an MI355X device (got %s); this path has no CPU implementation" % (name, t.device))
+    if t.dtype not in _DTYPE_CODES:
+        raise TypeError("%s must be float32, float16 or bfloat16 (got %s)" % (name, t.dtype))
+    if t.get_device() != torch.cuda.current_device():
+        raise RuntimeError("%s lives on %s but the current device is cuda:%d (use torch.cuda.set_device / torch.cuda.device)"
+                           % (name, t.device, torch.cuda.current_device()))
+    return t
+
+
+def _row_strides(t):
+    """(sample stride, row stride) of a channels-last tensor [N, ..., C] whose positions lie at one distance, as in a dense tensor
+    or in a channel slice of a wider one; None if they do not (or channels are not consecutive)."""
+    shape, st = t.shape, t.stride()
+    if t.is_contiguous():
+        return (t.numel() // max(shape[0], 1), shape[-1])
+    if shape[-1] != 1 and st[-1] != 1:
+        return None
+    row = expected = None
+    for i in range(t.dim() - 2, 0, -1):
+        if shape[i] == 1:
+            continue
+        if row is None:
+            row = expected = st[i]
+        elif st[i] != expected:
+            return None
+        expected *= shape[i]
+    return (st[0], 0 if row is None else row)
+
+
+def _rows(t):
+    """t as the kernels read it, and its strides: itself, or a contiguous copy."""
+    strides = _row_strides(t)
+    if strides is None:
+        t = t.contiguous()
+        strides = _row_strides(t)
+    return t, strides
+
+
+def _extent(t):
+    """[first byte, behind the last byte) of a tensor's values."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_out(out, t, name):
+    """out may be t itself or lie beside it (also as another channel slice of the same rows), not across it."""
+    if t is None or not out.numel():
+        return
+    (a, b), (c, d) = _extent(out), _extent(t)
+    if a >= d or c >= b or (a == c and out.stride() == t.stride() and out.shape == t.shape):
+        return
+    so, width = _row_strides(out), out.shape[-1]
+    if so == _row_strides(t) and so[1] and (out.shape[0] == 1 or so[0] % so[1] == 0):
+        gap = (c - a) // out.element_size() % so[1]
+        if width <= gap <= so[1] - width:
+            return
+    raise ValueError("out overlaps %s: pass %s itself, or memory of its own" % (name, name))
+
+
+def _check_norm_args(x, groups, weight, bias, eps, act, residual):
+    _require_gpu(x, "x")
+    if x.dim() < 2:
+        raise ValueError("x must be channels-last [N, ..., C] (got %s)" % (tuple(x.shape),))
+    c = x.shape[-1]
+    if isinstance(groups, bool) or int(groups) != groups or groups < 1 or c < 1 or c % int(groups):
+        raise ValueError("groups=%r does not divide the %d channels" % (groups, c))
+    if act not in _ACT_CODES:
+        raise ValueError("act must be one of %s (got %r)" % (tuple(_ACT_CODES), act))
+    if not 0 <= eps < float("inf"):
+        raise ValueError("eps must be finite and not negative (got %r)" % (eps,))
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            _require_gpu(p, name)
+            if tuple(p.shape) != (c,):
+                raise ValueError("%s must be [%d] (got %s)" % (name, c, tuple(p.shape)))
+    if residual is not None:
+        _require_gpu(residual, "residual")
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("residual %s %s differs from x %s %s" % (residual.dtype, tuple(residual.shape), x.dtype, tuple(x.shape)))
+
+
+def _norm_dims(x, groups):
+    n, c = x.shape[0], x.shape[-1]
+    return n, (x.numel() // (n * c) if n else 0), c, int(groups)
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+def _group_norm_forward(x, groups, weight, bias, eps, act, residual, y, stats, workspace=_workspace):
+    """One msnet_group_norm call into y; x and residual as _rows gives them."""
+    n, s, c, g = _norm_dims(x, groups)
+    lib, code, xs, ys = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(y)
+    rs = _row_strides(residual) if residual is not None else (0, 0)
+    nbytes = lib.msnet_group_norm_workspace_bytes(code, n, s, c, g)
+    ws = workspace(nbytes, x.device)
+    check(lib.msnet_group_norm(ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y), ptr(stats), code, _ACT_CODES[act], n, s, c, g, eps,
+                               xs[0], xs[1], rs[0], rs[1], ys[0], ys[1], ptr(ws), nbytes, stream_ptr()), "msnet_group_norm")
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, groups, eps, act):
+        x, _ = _rows(x)
+        if residual is not None:
+            residual, _ = _rows(residual)
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        stats = torch.empty((x.shape[0], groups, 2), device=x.device, dtype=torch.float64)
+        _group_norm_forward(x, groups, weight, bias, eps, act, residual, y, stats)
+        ctx.groups, ctx.act = groups, act
+        ctx.save_for_backward(x, weight, bias, residual if act != "none" else None, stats)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, residual, stats = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dy, ds = _rows(dy)
+        xs = _row_strides(x)
+        rs = _row_strides(residual) if residual is not None else (0, 0)
+        n, s, c, g = _norm_dims(x, ctx.groups)
+        new = lambda wanted, shape, dtype: torch.empty(shape, device=x.device, dtype=dtype) if wanted else None      # noqa: E731
+        dx = new(need_x, x.shape, x.dtype)
+        dres = new(need_r and ctx.act != "none", x.shape, x.dtype)
+        dw, db = new(need_w, (c,), torch.float32), new(need_b, (c,), torch.float32)
+        lib, code = _lib.load(), _DTYPE_CODES[x.dtype]
+        nbytes = lib.msnet_group_norm_backward_workspace_bytes(code, n, s, c, g)
+        ws = _workspace(nbytes, x.device)
+        check(lib.msnet_group_norm_backward(ptr(dy), ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(stats), ptr(dx), ptr(dres), ptr(dw), ptr(db),
+                                            code, _ACT_CODES[ctx.act], n, s, c, g, ds[0], ds[1], xs[0], xs[1], rs[0], rs[1], ptr(ws), nbytes,
+                                            stream_ptr()), "msnet_group_norm_backward")
+        return dx, dw, db, (dy if need_r and ctx.act == "none" else dres), None, None, None
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual=None, out=None):
+    """act(group_norm(x) * weight + bias (+ residual)) over a channels-last x [N, ..., C] (NDHWC activations, or [N, rows, C]):
+    mean and variance over all positions and the C / groups channels of one sample and group.  x, residual and the result are
+    float32, float16 or bfloat16; weight and bias [C] of any of these; sums are 64-bit.  act: "none", "relu" or "silu".  Channel
+    slices of wider tensors are taken as they are, other strides are copied.  out: where the result goes -- x or residual
+    themselves, or memory beside them; only where no gradient is asked for.
+
+    With gradients enabled the result is differentiable once in x, weight, bias and residual; x, the residual (with an activation)
+    and 16 bytes a sample and group are kept for it.  Results and gradients repeat bit for bit.  Inside a forward of the aggregators
+    the result raises the fp16-range flag as a conv's does (RangeGuard)."""
+    _check_norm_args(x, groups, weight, bias, eps, act, residual)
+    groups, eps = int(groups), float(eps)
+    if weight is not None and (weight.dtype != torch.float32 or not weight.is_contiguous()):
+        weight = weight.float().contiguous()
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.float().contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        if out is not None:
+            raise ValueError("out cannot be used where a gradient is asked for")
+        return _GroupNorm.apply(x, weight, bias, residual, groups, eps, act)
+    x, _ = _rows(x)
+    if residual is not None:
+        residual, _ = _rows(residual)
+    arena = _tls.arena is not None and x.dtype == torch.float32
+    if out is None:
+        out = _new(x.shape, x.device) if arena else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    else:
+        _require_gpu(out, "out")
+        strides, (n, s, c, _) = _row_strides(out), _norm_dims(x, groups)
+        if out.shape != x.shape or out.dtype != x.dtype or strides is None or (s > 1 and strides[1] < c) or (n > 1 and strides[0] < (s - 1) * strides[1] + c):
+            raise ValueError("out must be %s %s with consecutive channels and evenly spaced rows of its own" % (x.dtype, tuple(x.shape)))
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out must not require a gradient")
+        _check_out(out, x, "x")
+        _check_out(out, residual, "residual")
+    _group_norm_forward(x, groups, weight, bias, eps, act, residual, out, None,
+                        (lambda nbytes, dev: _new(((nbytes + 3) // 4,), dev) if nbytes else None) if arena else _workspace)
+    return out
+
+
+# ---- gradient norm and clipping -------------------------------------------------------------------------------------------
+
+def _is_dense(t):
+    """Whether t's values fill its memory from first to last, in whatever order of dimensions (a channels-last weight's gradient)."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expected:
+            return False
+        expected *= n
+    return True
+
+
+def _clip(grads, max_norm, outs):
+    """One msnet_clip_grads call over dense tensors (outs None: the norm alone)."""
+    from array import array
+    dev = torch.device("cuda", torch.cuda.current_device())
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    pointers = lambda ts: array("Q", [t.data_ptr() for t in ts])                      # noqa: E731
+    types = lambda ts: bytes([_DTYPE_CODES[t.dtype] for t in ts])                     # noqa: E731
+    src, lengths, stypes = pointers(grads), array("q", [t.numel() for t in grads]), types(grads)
+    dst, dtypes = (src, stypes) if outs is grads else (pointers(outs), types(outs)) if outs is not None else (None, None)
+    addr = lambda a: a.buffer_info()[0] if a is not None else None                     # noqa: E731
+    lib = _lib.load()
+    nbytes = lib.msnet_clip_grads_workspace_bytes(addr(lengths), len(grads))
+    ws = _workspace(nbytes, dev)
+    check(lib.msnet_clip_grads(addr(src), addr(dst), addr(lengths), stypes, dtypes, len(grads), max_norm, ptr(norm), ptr(ws), nbytes, stream_ptr()),
+          "msnet_clip_grads")
+    return norm
+
+
+def _grad_list(grads, name):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    for i, t in enumerate(grads):
+        _require_gpu(t, "%s[%d]" % (name, i))
+    return grads
+
+
+def grad_norm(grads):
+    """The 2-norm over all values of all the given tensors (float32, float16, bfloat16, any shapes and mix): a float32 scalar on the
+    device, nothing waits for it.  Squares are formed and added in 64 bits."""
+    grads = _grad_list(grads, "grads")
+    return _clip([t.detach() if _is_dense(t) else t.detach().contiguous() for t in grads], 0.0, None)
+
+
+def clip_grads(grads, max_norm, out=None):
+    """Scales the gradients by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of them (grad_norm), and returns the norm:
+    in place, or into `out`, one tensor a gradient of its shape, of its type or float32.  Gradients that are short enough are left
+    as they are (in place nothing is written).  The host is never asked: an infinite norm scales finite values to 0, and a NaN among
+    the gradients makes all of them NaN.  A tensor listed twice, or one that overlaps another, is refused where it would be written."""
+    grads = _grad_list(grads, "grads")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be negative (got %r)" % (max_norm,))
+    if out is None:
+        outs = grads
+    else:
+        outs = _grad_list(out, "out")
+        if len(outs) != len(grads):
+            raise ValueError("%d gradients, %d outputs" % (len(grads), len(outs)))
+        for i, (t, o) in enumerate(zip(grads, outs)):
+            if o.shape != t.shape or (o.dtype != t.dtype and o.dtype != torch.float32):
+                raise ValueError("out[%d] must be %s, %s or float32 (got %s %s)" % (i, tuple(t.shape), t.dtype, o.dtype, tuple(o.shape)))
+    if torch.is_grad_enabled() and any(o.requires_grad for o in outs):
+        raise ValueError("a tensor to be written requires a gradient itself")
+    src, dst, back = grads, outs, []
+    if not all(_is_dense(t) and _is_dense(o) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())) for t, o in zip(grads, outs)):
+        src, dst = [], []
+        for t, o in zip(grads, outs):                       # a value's place in memory has to be the same on both sides
+            same = t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())
+            if same and _is_dense(t):
+                src.append(t)
+                dst.append(o)
+            else:
+                if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+                    raise ValueError("a tensor to be written is expanded: its values share memory")
+                src.append(t.contiguous())
+                dst.append(torch.empty_like(src[-1], dtype=o.dtype))
+                back.append((o, dst[-1]))
+    norm = _clip(src, max_norm, src if dst is grads else dst)
+    for o, d in back:
+        o.copy_(d)
+    torch.autograd.graph.increment_version(outs)            # written behind autograd's back: what saved them finds out
+    return norm
+
+
 class _ActiveGuard(threading.local):
     guard = None
 
