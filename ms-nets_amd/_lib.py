@@ -8,6 +8,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # MSNET_HIP_LIB lets an A/B experiment point at another build of the same ABI (tools_layer_bench.py)
 LIB_PATH = os.environ.get("MSNET_HIP_LIB") or os.path.join(_HERE, "libmsnet_hip.so")
 _lib = None
+_host = None
 
 
 class VolumeParams(ctypes.Structure):
@@ -121,6 +122,20 @@ def load():
         raise RuntimeError("libmsnet_hip.so ABI version %d != 1" % lib.msnet_version())
     _lib = lib
     return lib
+
+
+def load_host():
+    """The Python module _host (csrc/host_tables.cpp), loaded once; raises RuntimeError if it is not built."""
+    global _host
+    if _host is None:
+        import torch  # noqa: F401  (its libraries are what the module is linked against)
+        import importlib
+        try:
+            _host = importlib.import_module(__package__ + "._host")
+        except ImportError as e:
+            raise RuntimeError("ms-nets_amd/_host.so is not built or does not load (%s). Run `python -c 'import __graft_entry__ as g; "
+                               "g.build()'`" % e) from e
+    return _host
 
 
 def check(rc, what):

@@ -12,6 +12,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmsnet_hip.so")
+HOST = os.path.join(HERE, "_host.so")                 # Python module: reads lists of tensors (csrc/host_tables.cpp)
 ARCH = "gfx950"
 
 # gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself.
@@ -152,6 +153,29 @@ def _build_locked(hipcc, objdir, out, force, verbose, defines):
     return out
 
 
+def build_host(force=False, verbose=True):
+    """The Python module _host (csrc/host_tables.cpp): host code against torch's headers, g++ alone."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "host_tables.cpp")
+    libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    for inc in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]:
+        flags += ["-isystem", inc]
+    links = ["-L" + libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    digest = _digest([src], flags + links + [torch.__version__, sys.version])
+    if force or _stale(HOST, HOST + ".sha", digest):
+        tmp = "%s.%d.tmp" % (HOST, os.getpid())
+        cmd = ["g++"] + flags + [src, "-o", tmp] + links
+        if verbose:
+            print("[build]", " ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+        os.replace(tmp, HOST)
+        _write_stamp(HOST + ".sha", digest)
+    return HOST
+
+
 build.last_compiled = []
 
 
@@ -159,3 +183,5 @@ if __name__ == "__main__":
     defs = [a[2:] for a in sys.argv[1:] if a.startswith("-D")]
     out = [a[6:] for a in sys.argv[1:] if a.startswith("--lib=")]
     build(force="--force" in sys.argv, defines=defs, lib=out[0] if out else None)
+    if not out:
+        build_host(force="--force" in sys.argv)

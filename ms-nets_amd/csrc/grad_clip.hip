@@ -3,10 +3,11 @@
 //   norm = sqrt(sum over all tensors of sum g^2),   out = g * min(1, max_norm / (norm + 1e-6))
 //
 // Memory-bound twice over: the norm has to be known before the first value is scaled, so gradients larger than the caches are read
-// twice.  The table of tensors travels in the kernels' arguments (nothing is uploaded, a captured graph keeps it); a workgroup takes
-// one chunk of one tensor and finds it by bisection.  grad_square_sums writes one 64-bit sum a workgroup, grad_scale adds all of
-// them up in a fixed order at its start: two launches for kTensors tensors, no atomics, and a result repeats bit for bit.
-// Squares are formed and added in 64 bits, so no gradient's square overflows or vanishes.
+// twice.  Tensors are cut into chunks of kChunk values, and the workgroups take chunks in turn, so that all of them together stream
+// through one window of memory.  Up to kTensors tensors travel in the kernels' own arguments; more are written to the workspace
+// first, kPart a launch, with every chunk's tensor beside them (so a captured graph needs no host memory either way).
+// grad_square_sums leaves one 64-bit sum a workgroup, and each workgroup of grad_scale adds all of them up in a fixed order: no
+// atomics, and a result repeats bit for bit.  Squares are formed and added in 64 bits, so no gradient's square overflows or vanishes.
 #include <algorithm>
 #include <vector>
 
@@ -16,31 +17,83 @@ namespace msnet {
 namespace clip {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 112;          // of one launch: the table keeps below the 4 KB of kernel arguments
-constexpr long kChunk = 8192;          // values of a workgroup at least
-constexpr long kBlocks = 2048;         // workgroups of a call beyond one a tensor, at most
+constexpr int kTensors = 112;          // in a kernel's arguments, which are 4 KB at most
+constexpr int kPart = 140;             // of one launch that writes them to the workspace
+constexpr int kChunk = 16384;          // values of a chunk
+constexpr unsigned kBlocks = 1024;     // workgroups at most: four a compute unit, all on the device at once
 
-struct Table {
-    const void* in[kTensors];
-    void* out[kTensors];
-    long n[kTensors];
-    unsigned first[kTensors + 1];      // first workgroup of each tensor
-    unsigned char types[kTensors];     // input's type + 4 * output's
+// One tensor.  n: its length, its input's type in bits 60 and 61, its output's in the top two.
+struct Entry { const void* in; void* out; unsigned long n; };
+__host__ __device__ inline unsigned long packed(long n, int in, int out) { return (unsigned long)n | (unsigned long)in << 60 | (unsigned long)out << 62; }
+__device__ __forceinline__ long length(const Entry& e) { return (long)(e.n & ((1ul << 60) - 1)); }
+__device__ __forceinline__ int types(const Entry& e) { return (int)(e.n >> 60); }      // input's + 4 * output's
+
+struct Arguments {
+    Entry e[kTensors];
+    unsigned first[kTensors + 1];      // first chunk of each tensor
     int count;
 };
-static_assert(sizeof(Table) + 64 <= 4096, "kernel arguments");
+
+// Where a workgroup finds its chunks' tensors: the arguments, which lie in host memory, are copied to LDS at once, and a chunk's
+// tensor is the number of first chunks up to it, two a lane.
+struct ArgumentLookup {
+    Entry* e;
+    unsigned a, b;
+    __device__ __forceinline__ ArgumentLookup(const Arguments& t, Entry* lds) : e(lds) {
+        static_assert(kTensors <= 128, "two a lane");
+        const int tid = threadIdx.x, lane = tid & 63;
+        if (tid < t.count) lds[tid] = t.e[tid];
+        a = lane < t.count ? t.first[lane] : ~0u;
+        b = lane + 64 < t.count ? t.first[lane + 64] : ~0u;
+        __syncthreads();
+    }
+    __device__ __forceinline__ Entry find(unsigned chunk, long* at) const {
+        const int k = __popcll(__ballot(a <= chunk)) + __popcll(__ballot(b <= chunk)) - 1;
+        const unsigned first = k < 64 ? __shfl(a, k) : __shfl(b, k - 64);
+        *at = (long)(chunk - first) * kChunk;
+        return e[k];
+    }
+};
+
+struct Workspace {
+    const Entry* e;
+    const unsigned* first;
+    const unsigned* tensor;            // of each chunk
+};
+
+struct WorkspaceLookup {
+    Workspace w;
+    __device__ __forceinline__ WorkspaceLookup(const Workspace& t, Entry*) : w(t) {}
+    __device__ __forceinline__ Entry find(unsigned chunk, long* at) const {
+        const unsigned k = w.tensor[chunk];
+        *at = (long)(chunk - w.first[k]) * kChunk;
+        return w.e[k];
+    }
+};
+
+template <class Source> struct Lookup;
+template <> struct Lookup<Arguments> { typedef ArgumentLookup type; };
+template <> struct Lookup<Workspace> { typedef WorkspaceLookup type; };
+
+struct Part {
+    Entry e[kPart];
+    unsigned first[kPart + 1];
+    int count;
+};
+static_assert(sizeof(Arguments) + 64 <= 4096 && sizeof(Part) + 64 <= 4096, "kernel arguments");
+
+__global__ __launch_bounds__(kThreads) void grad_table(Part p, int at, Entry* __restrict__ e, unsigned* __restrict__ first, unsigned* __restrict__ tensor) {
+    __shared__ unsigned begin[kPart + 1];
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (tid < p.count) { e[at + tid] = p.e[tid]; first[at + tid] = p.first[tid]; }      // (the arguments lie in host memory: one wait for all)
+    if (tid <= p.count) begin[tid] = p.first[tid];
+    __syncthreads();
+    for (int i = tid >> 6; i < p.count; i += kThreads / 64)
+        for (unsigned b = begin[i] + lane; b < begin[i + 1]; b += 64) tensor[b] = (unsigned)(at + i);
+}
+static_assert(kPart < kThreads, "one thread a tensor");
 
 template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };      // any view's alignment
-
-__device__ __forceinline__ int tensor_of(const Table& t, unsigned block) {
-    int lo = 0, hi = t.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (t.first[mid] <= block) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
 
 __device__ __forceinline__ double block_sum(double s, double* tab, int tid) {
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -50,15 +103,15 @@ __device__ __forceinline__ double block_sum(double s, double* tab, int tid) {
 }
 
 template <class T>
-__device__ __forceinline__ double square_sum(const T* p, long n, int tid) {
+__device__ __forceinline__ double square_sum(const T* p, int n, int tid) {
     constexpr int V = 16 / sizeof(T);
     typedef typename Pack<T, V>::type Vec;
     double s[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = 0.;
-    const long nv = n / V;
+    const int nv = n / V;
     const Vec* v = reinterpret_cast<const Vec*>(p);
-    long i = tid;
+    int i = tid;
     auto add = [&](const Vec& a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -74,85 +127,117 @@ __device__ __forceinline__ double square_sum(const T* p, long n, int tid) {
     double r = s[0];
 #pragma unroll
     for (int e = 1; e < V; ++e) r += s[e];
-    const long at = nv * V + tid;
+    const int at = nv * V + tid;
     if (at < n) { const double d = (double)(float)p[at]; r = fma(d, d, r); }
     return r;
 }
 
-__global__ __launch_bounds__(kThreads) void grad_square_sums(Table t, long chunk, double* __restrict__ sums) {
+template <class Source>
+__global__ __launch_bounds__(kThreads) void grad_square_sums(Source src, unsigned chunks, double* __restrict__ sums) {
     __shared__ double tab[4];
-    const int tid = threadIdx.x, k = tensor_of(t, blockIdx.x);
-    const long at = (long)(blockIdx.x - t.first[k]) * chunk, n = min(chunk, t.n[k] - at);
-    double s;
-    switch (t.types[k] & 3) {
-        case 0: s = square_sum(static_cast<const float*>(t.in[k]) + at, n, tid); break;
-        case 1: s = square_sum(static_cast<const _Float16*>(t.in[k]) + at, n, tid); break;
-        default: s = square_sum(static_cast<const __bf16*>(t.in[k]) + at, n, tid);
+    __shared__ Entry lds[kTensors];
+    const int tid = threadIdx.x;
+    const typename Lookup<Source>::type table(src, lds);
+    double s = 0.;
+    for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
+        long at;
+        const Entry e = table.find(c, &at);
+        const int n = (int)min((long)kChunk, length(e) - at);
+        switch (types(e) & 3) {
+            case 0: s += square_sum(static_cast<const float*>(e.in) + at, n, tid); break;
+            case 1: s += square_sum(static_cast<const _Float16*>(e.in) + at, n, tid); break;
+            default: s += square_sum(static_cast<const __bf16*>(e.in) + at, n, tid);
+        }
     }
     s = block_sum(s, tab, tid);
     if (tid == 0) sums[blockIdx.x] = s;
 }
 
+__device__ __forceinline__ double total_of(const double* __restrict__ sums, unsigned n, double* tab, int tid) {
+    double s = 0.;
+#pragma unroll 4
+    for (unsigned i = tid; i < n; i += kThreads) s += sums[i];
+    return block_sum(s, tab, tid);
+}
+
+// One workgroup: the norm alone.
+__global__ __launch_bounds__(kThreads) void grad_total(const double* __restrict__ sums, unsigned n, float* norm) {
+    __shared__ double tab[4];
+    const double s = total_of(sums, n, tab, threadIdx.x);
+    if (threadIdx.x == 0) *norm = (float)sqrt(s);
+}
+
 template <class T, class O>
-__device__ __forceinline__ void scale(const T* p, O* o, long n, float f, int tid) {
+__device__ __forceinline__ void scale(const T* p, O* o, int n, float f, int tid) {
     constexpr int V = 16 / sizeof(T);
     typedef typename Pack<T, V>::type Vec;
     typedef typename Pack<O, V>::type Out;
-    const long nv = n / V;
+    const int nv = n / V;
     const Vec* v = reinterpret_cast<const Vec*>(p);
     Out* w = reinterpret_cast<Out*>(o);
-    auto put = [&](long i, const Vec& a) {
+    auto put = [&](int i, const Vec& a) {
         Out r;
 #pragma unroll
         for (int e = 0; e < V; ++e) r[e] = (O)((float)a[e] * f);
         w[i] = r;
     };
-    long i = tid;
+    int i = tid;
     for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
         const Vec a = v[i], b = v[i + kThreads], c = v[i + 2 * kThreads], d = v[i + 3 * kThreads];
         put(i, a); put(i + kThreads, b); put(i + 2 * kThreads, c); put(i + 3 * kThreads, d);
     }
     for (; i < nv; i += kThreads) put(i, v[i]);
-    const long at = nv * V + tid;
+    const int at = nv * V + tid;
     if (at < n) o[at] = (O)((float)p[at] * f);
 }
 
-// norm: where the first launch's first workgroup leaves it, or null.  scaling: whether there is anything to scale.
-__global__ __launch_bounds__(kThreads) void grad_scale(Table t, long chunk, const double* __restrict__ sums, unsigned nsums, double max_norm,
-                                                       float* norm, int scaling) {
+template <class Source>
+__global__ __launch_bounds__(kThreads) void grad_scale(Source src, unsigned chunks, const double* __restrict__ sums, double max_norm, float* norm) {
     __shared__ double tab[4];
+    __shared__ Entry lds[kTensors];
     const int tid = threadIdx.x;
-    double s = 0.;
-#pragma unroll 4
-    for (unsigned i = tid; i < nsums; i += kThreads) s += sums[i];
-    const double total = sqrt(block_sum(s, tab, tid));
-    if (norm && blockIdx.x == 0 && tid == 0) *norm = (float)total;
-    if (!scaling) return;
+    const typename Lookup<Source>::type table(src, lds);
+    const double total = sqrt(total_of(sums, gridDim.x, tab, tid));
+    if (blockIdx.x == 0 && tid == 0) *norm = (float)total;
     const double r = max_norm / (total + 1e-6);
     const float f = r > 1. ? 1.f : (float)r;               // (a NaN stays one)
-    const int k = tensor_of(t, blockIdx.x);
-    if (f == 1.f && t.in[k] == t.out[k]) return;           // short enough already, in place
-    const long at = (long)(blockIdx.x - t.first[k]) * chunk, n = min(chunk, t.n[k] - at);
-    const void* p = t.in[k];
-    void* o = t.out[k];
-    switch (t.types[k]) {
-        case 0: scale(static_cast<const float*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-        case 1: scale(static_cast<const _Float16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-        case 2: scale(static_cast<const __bf16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-        case 5: scale(static_cast<const _Float16*>(p) + at, static_cast<_Float16*>(o) + at, n, f, tid); break;
-        default: scale(static_cast<const __bf16*>(p) + at, static_cast<__bf16*>(o) + at, n, f, tid);
+    // last chunks first: what the sums read last is what the caches hold
+    for (unsigned c = blockIdx.x + (chunks - 1 - blockIdx.x) / gridDim.x * gridDim.x;; c -= gridDim.x) {
+        long at;
+        const Entry e = table.find(c, &at);
+        if (f != 1.f || e.in != e.out) {                   // (else: short enough already, in place)
+            const int n = (int)min((long)kChunk, length(e) - at);
+            const void* p = e.in;
+            void* o = e.out;
+            switch (types(e)) {
+                case 0: scale(static_cast<const float*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 1: scale(static_cast<const _Float16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 2: scale(static_cast<const __bf16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 5: scale(static_cast<const _Float16*>(p) + at, static_cast<_Float16*>(o) + at, n, f, tid); break;
+                default: scale(static_cast<const __bf16*>(p) + at, static_cast<__bf16*>(o) + at, n, f, tid);
+            }
+        }
+        if (c < gridDim.x) break;
     }
 }
 
-// The workgroups of a call: chunk values each, more where the whole is large.
-struct Cut { long chunk; unsigned long blocks; };
+struct Cut {
+    unsigned long chunks;
+    int tensors;                       // that hold any value
+    unsigned blocks() const { return chunks < kBlocks ? (unsigned)chunks : kBlocks; }
+    size_t bytes() const {             // the sums, the tensors of a long list and the chunks'
+        return (size_t)kBlocks * sizeof(double) + (tensors > kTensors ? (size_t)tensors * (sizeof(Entry) + sizeof(unsigned)) + chunks * sizeof(unsigned) : 0);
+    }
+};
+
+static long chunks_of(int64_t n) { return (long)((n + kChunk - 1) / kChunk); }
 
 static Cut cut(const int64_t* n, int count) {
-    double total = 0;
-    for (int i = 0; i < count; ++i) total += (double)n[i];
-    Cut c = {kChunk, 0};
-    if (total > (double)kChunk * kBlocks) c.chunk = ((long)(total / kBlocks) / kChunk + 1) * kChunk;
-    for (int i = 0; i < count; ++i) c.blocks += (unsigned long)((n[i] + c.chunk - 1) / c.chunk);
+    Cut c = {0, 0};
+    for (int i = 0; i < count; ++i) {
+        c.chunks += (unsigned long)chunks_of(n[i]);
+        c.tensors += n[i] > 0;
+    }
     return c;
 }
 
@@ -193,7 +278,7 @@ static int check_lengths(const char* what, const int64_t* n, int count) {
 
 extern "C" size_t msnet_clip_grads_workspace_bytes(const int64_t* n_host, int count) {
     if (check_lengths("msnet_clip_grads_workspace_bytes", n_host, count)) return 0;
-    return (clip::cut(n_host, count).blocks + 1) * sizeof(double);
+    return clip::cut(n_host, count).bytes();
 }
 
 extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_host, const int64_t* n_host, const uint8_t* in_types_host,
@@ -203,9 +288,9 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
     if (!norm || (count && (!in_host || !in_types_host)) || (out_host && !out_types_host)) return fail("msnet_clip_grads: null pointer");
     if (out_host && !(max_norm >= 0.)) return fail("msnet_clip_grads: max_norm=%g", max_norm);
     const clip::Cut c = clip::cut(n_host, count);
-    if (c.blocks > 0x7ffffffful) return fail("msnet_clip_grads: %lu workgroups are too many", c.blocks);
-    if (!workspace || workspace_bytes < (c.blocks + 1) * sizeof(double) || ((uintptr_t)workspace & 7))
-        return fail("msnet_clip_grads: workspace of %zu bytes at %p, %zu needed", workspace_bytes, workspace, (size_t)((c.blocks + 1) * sizeof(double)));
+    if (c.chunks > 0x7ffffffful) return fail("msnet_clip_grads: %lu chunks are too many", c.chunks);
+    if (!workspace || workspace_bytes < c.bytes() || ((uintptr_t)workspace & 7))
+        return fail("msnet_clip_grads: workspace of %zu bytes at %p, %zu needed", workspace_bytes, workspace, c.bytes());
     for (int i = 0; i < count; ++i) {
         const int in = in_types_host[i], out = out_host ? out_types_host[i] : in;
         if (in > 2 || (out != in && out != 0)) return fail("msnet_clip_grads: tensor %d: types %d to %d (0 float32, 1 float16, 2 bfloat16; out: the same or float32)", i, in, out);
@@ -224,37 +309,60 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
         bytes_in += (double)n_host[i] * (in_types_host[i] ? 2 : 4);
         if (out_host) bytes_out += (double)n_host[i] * (out_types_host[i] ? 2 : 4);
     }
-    // pass 0: the sums; pass 1: the scaled gradients (or the norm alone).  Both cut the tensors the same way.
-    for (int pass = 0; pass < 2; ++pass) {
-        LaunchScope ls(pass ? "grad_scale" : "grad_square_sums", s, 0, pass ? bytes_out + (out_host ? bytes_in : 0.) : bytes_in);
-        clip::Table t;
-        unsigned long done = 0;                             // workgroups of this pass's earlier launches
-        bool first = true;
-        t.count = 0;
-        t.first[0] = 0;
-        for (int i = 0; i <= count; ++i) {
-            if (i < count && n_host[i]) {
-                t.in[t.count] = in_host[i];
-                t.out[t.count] = out_host ? out_host[i] : nullptr;
-                t.n[t.count] = n_host[i];
-                t.types[t.count] = (unsigned char)(in_types_host[i] + 4 * (out_host ? out_types_host[i] : in_types_host[i]));
-                t.first[t.count + 1] = t.first[t.count] + (unsigned)((n_host[i] + c.chunk - 1) / c.chunk);
-                ++t.count;
-            }
-            if (t.count < clip::kTensors && i < count) continue;
-            const unsigned blocks = t.first[t.count];
-            if (pass == 0 && blocks)
-                hipLaunchKernelGGL(clip::grad_square_sums, dim3(blocks), dim3(clip::kThreads), 0, s, t, c.chunk, sums + done);
-            if (pass == 1 && ((blocks && out_host) || first)) {
-                const bool scaling = blocks && out_host;
-                hipLaunchKernelGGL(clip::grad_scale, dim3(scaling ? blocks : 1), dim3(clip::kThreads), 0, s, t, c.chunk, sums, (unsigned)c.blocks, max_norm,
-                                   first ? norm : nullptr, (int)scaling);
-                first = false;
-            }
-            if (int rc = check_launch("msnet_clip_grads")) return rc;
-            done += blocks;
-            t.count = 0;
+    const unsigned blocks = c.blocks(), chunks = (unsigned)c.chunks;
+    const auto entry = [&](int i) {
+        return clip::Entry{in_host[i], out_host ? out_host[i] : nullptr,
+                           clip::packed(n_host[i], in_types_host[i], out_host ? out_types_host[i] : in_types_host[i])};
+    };
+    const auto run = [&](auto src) {
+        if (blocks) {
+            LaunchScope ls("grad_square_sums", s, 0, bytes_in);
+            hipLaunchKernelGGL((clip::grad_square_sums<decltype(src)>), dim3(blocks), dim3(clip::kThreads), 0, s, src, chunks, sums);
         }
+        if (out_host && blocks) {
+            LaunchScope ls("grad_scale", s, 0, bytes_in + bytes_out);
+            hipLaunchKernelGGL((clip::grad_scale<decltype(src)>), dim3(blocks), dim3(clip::kThreads), 0, s, src, chunks, sums, max_norm, norm);
+        } else {
+            LaunchScope ls("grad_total", s, 0, 8.0 * blocks);
+            hipLaunchKernelGGL(clip::grad_total, dim3(1), dim3(clip::kThreads), 0, s, sums, blocks, norm);
+        }
+        return check_launch("msnet_clip_grads");
+    };
+    if (c.tensors <= clip::kTensors) {
+        clip::Arguments a;
+        a.count = 0;
+        a.first[0] = 0;
+        for (int i = 0; i < count; ++i)
+            if (n_host[i]) {
+                a.e[a.count] = entry(i);
+                a.first[a.count + 1] = a.first[a.count] + (unsigned)clip::chunks_of(n_host[i]);
+                ++a.count;
+            }
+        return run(a);
     }
-    return 0;
+    clip::Entry* e = reinterpret_cast<clip::Entry*>(sums + clip::kBlocks);
+    unsigned* first = reinterpret_cast<unsigned*>(e + c.tensors);
+    unsigned* tensor = first + c.tensors;
+    {
+        LaunchScope ls("grad_table", s, 0, 28.0 * c.tensors + 4.0 * chunks);
+        clip::Part p;
+        p.count = 0;
+        p.first[0] = 0;
+        int at = 0;
+        for (int i = 0; i < count; ++i) {
+            if (n_host[i]) {
+                p.e[p.count] = entry(i);
+                p.first[p.count + 1] = p.first[p.count] + (unsigned)clip::chunks_of(n_host[i]);
+                ++p.count;
+            }
+            if (p.count == clip::kPart || (i == count - 1 && p.count)) {
+                hipLaunchKernelGGL(clip::grad_table, dim3(1), dim3(clip::kThreads), 0, s, p, at, e, first, tensor);
+                at += p.count;
+                p.first[0] = p.first[p.count];
+                p.count = 0;
+            }
+        }
+        if (int rc = check_launch("msnet_clip_grads")) return rc;
+    }
+    return run(clip::Workspace{e, first, tensor});
 }

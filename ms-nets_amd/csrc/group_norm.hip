@@ -40,18 +40,17 @@ Shape make_shape(int N, long S, int C, int G, int* V, long most_cw) {
         s.chunks = (G + s.gpc - 1) / s.gpc;
         s.nsub = 1; s.cw = (s.gpc < G ? s.gpc : G) * s.cg;
     }
-    s.nblk = 1; s.rows = S;
+    s.nblk = 1;
     return s;
 }
 
-void cut_rows(Shape* s, int V, long most_blocks, int least_passes) {
-    const long per_pass = kThreads / (s->cw / V), least = per_pass * least_passes;
-    long nblk = most_blocks / ((long)s->N * s->chunks);
-    if (nblk > (s->S + least - 1) / least) nblk = (s->S + least - 1) / least;
-    if (nblk < 1) nblk = 1;
-    s->rows = ((s->S + nblk - 1) / nblk + per_pass - 1) / per_pass * per_pass;
-    s->nblk = (int)((s->S + s->rows - 1) / s->rows);
+void cut_rows(Shape* s, int V, long most_blocks, int tile, int tiles) {
+    const long least = (long)(kThreads / (s->cw / V)) * tile * tiles;
+    const long most = (s->S + least - 1) / least, nblk = most_blocks / ((long)s->N * s->chunks);
+    s->nblk = (int)(nblk < 1 ? 1 : nblk < most ? nblk : most);
 }
+
+constexpr int kTile = 4;               // rows a thread loads at once
 
 // mean and 1 / sqrt(var + eps) from the sums of x - pivot and of its square over m values
 __device__ __forceinline__ double2 statistics(double2 sum, double pivot, double m, double eps) {
@@ -127,7 +126,6 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict
         for (int g = tid; g < k.ng; g += kThreads) pivots[(size_t)k.n * sh.G + k.g0 + g] = (double)(float)xn[(size_t)(k.g0 + g) * sh.cg];
     if (row < per_pass) {
         const T* p = xn + k.c0 + cl;
-        long r = k.r0 + row;
         auto add = [&](const typename Pack<T, V>::type& v) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -136,14 +134,15 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict
                 q[e] = fma(d, d, q[e]);
             }
         };
-        for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {       // four loads in flight a thread
-            typename Pack<T, V>::type v[4];
+        walk<kTile, false>(sh, k.blk, row, per_pass,
+            [&](long r) {
+                typename Pack<T, V>::type v[kTile];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = load_raw<T, V>(p + (size_t)(r + (long)u * per_pass) * xr.ss);
+                for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(p + (size_t)(r + (long)u * per_pass) * xr.ss);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) add(v[u]);
-        }
-        for (; r < k.r1; r += per_pass) add(load_raw<T, V>(p + (size_t)r * xr.ss));
+                for (int u = 0; u < kTile; ++u) add(v[u]);
+            },
+            [&](long r) { add(load_raw<T, V>(p + (size_t)r * xr.ss)); });
         put_sums<V>(tab, tid, whole, s, q);
     }
     const int cols = whole ? cv : k.cw;
@@ -161,8 +160,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
                                                              double m, double eps, unsigned* oflag) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics
     double2* st = tab + kThreads;
-    // last rows first: what the sums read last is what the caches still hold
-    const Chunk k = chunk_of(sh, gridDim.x - 1 - blockIdx.x);
+    const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V;
     sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid, [&](int g, double2 sum) {
@@ -179,26 +177,25 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
     const long rs = residual ? rr.ss : xr.ss;
     T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
     unsigned amax = 0u;
-    long r = k.r0 + row;
-    for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {
-        typename Pack<T, V>::type v[4], w[4];
+    walk<kTile, true>(sh, k.blk, row, per_pass,                       // last rows first: what the sums read last is what the caches hold
+        [&](long r) {
+            typename Pack<T, V>::type v[kTile], w[kTile];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
-        if (residual)
+            for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+            if (residual)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
-        else
+                for (int u = 0; u < kTile; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+            else
 #pragma unroll
-            for (int u = 0; u < 4; ++u) w[u] = v[u];
+                for (int u = 0; u < kTile; ++u) w[u] = v[u];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, oflag != nullptr, amax);
-    }
-    for (; r < k.r1; r += per_pass) {
-        const auto v = load_raw<T, V>(px + (size_t)r * xr.ss);
-        const auto w = load_raw<T, V>(pr + (size_t)r * rs);
-        finish<T, V, ACT>(a, v, w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
-    }
+            for (int u = 0; u < kTile; ++u)
+                finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, oflag != nullptr, amax);
+        },
+        [&](long r) {
+            finish<T, V, ACT>(a, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pr + (size_t)r * rs), residual != nullptr, py + (size_t)r * yr.ss,
+                              oflag != nullptr, amax);
+        });
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);            // |y| >= 32752, inf or NaN: as the convs' epilogues
 }
 
@@ -279,7 +276,8 @@ struct Forward {
     hipStream_t stream;
 };
 
-constexpr long kStatsBlocks = 512, kApplyBlocks = 2048;
+constexpr long kStatsBlocks = 512, kApplyBlocks = 512;
+constexpr int kStatsTiles = 2, kApplyTiles = 2;      // tiles of a workgroup at least
 
 // One workgroup a chunk: threads and vectors a thread, or 0 where the chunk does not fit.
 static int small_threads(const Shape& s, int V, int* M) {
@@ -320,7 +318,7 @@ static Plan plan_forward(int N, long S, int C, int G, int dtype) {
     if (!p.threads) {
         p.V = vector_width(C, dtype);
         p.shape = make_shape(N, S, C, G, &p.V, 1l << 40);
-        cut_rows(&p.shape, p.V, kStatsBlocks, 8);
+        cut_rows(&p.shape, p.V, kStatsBlocks, kTile, kStatsTiles);
         p.bytes = stats_bytes(p.shape);
     }
     return p;
@@ -352,7 +350,7 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
         if (int rc = check_launch("msnet_group_norm")) return rc;
     }
     Shape out = sh;
-    cut_rows(&out, V, kApplyBlocks, 4);
+    cut_rows(&out, V, kApplyBlocks, kTile, kApplyTiles);
     const long grid2 = (long)out.N * out.nblk * out.chunks;
     LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
     hipLaunchKernelGGL((group_norm_apply<T, V, ACT>), dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr,

@@ -42,7 +42,9 @@ int backward_bf16(const Backward& f, const BackwardPlan& p, int act, void* ws);
 constexpr int kGradFew = 2;
 constexpr int grad_many(int V) { return V == 8 ? 4 : 8; }
 constexpr int kParamCols = 16;         // channels of one workgroup that sums dgamma and dbeta
-constexpr long kGradSumBlocks = 512, kGradApplyBlocks = 2048;
+constexpr long kGradSumBlocks = 512, kGradApplyBlocks = 512;
+constexpr int kSumTile = 4, kGradTile = 2;             // rows a thread loads at once
+constexpr int kGradSumTiles = 2, kGradApplyTiles = 2;  // tiles of a workgroup at least
 
 // What a thread keeps of its V channels.
 template <int V>
@@ -162,21 +164,22 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
                 q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
             }
         };
-        long r = k.r0 + row;
-        for (; r + 3l * per_pass < k.r1; r += 4l * per_pass) {
-            typename Pack<T, V>::type vx[4], vd[4], vr[4];
+        walk<kSumTile, false>(sh, k.blk, row, per_pass,
+            [&](long r) {
+                typename Pack<T, V>::type vx[kSumTile], vd[kSumTile], vr[kSumTile];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
-                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
-                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
-                else vr[u] = vx[u];
-            }
+                for (int u = 0; u < kSumTile; ++u) {
+                    vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+                    vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
+                    if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+                    else vr[u] = vx[u];
+                }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) add(vx[u], vd[u], vr[u]);
-        }
-        for (; r < k.r1; r += per_pass)
-            add(load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+                for (int u = 0; u < kSumTile; ++u) add(vx[u], vd[u], vr[u]);
+            },
+            [&](long r) {
+                add(load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+            });
 #pragma unroll
         for (int e = 0; e < V; ++e) tab[tid * V + e] = make_double2(s[e], q[e]);
     }
@@ -201,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
         param_grads(chan, chan_rows, sh.C, blockIdx.x, dweight, dbias, tab);
         return;
     }
-    const Chunk k = chunk_of(sh, gridDim.x - 1 - blockIdx.x);          // last rows first, as in the forward
+    const Chunk k = chunk_of(sh, blockIdx.x - param_blocks);
     double2 *st = tab + kThreads, *coef = st + k.ng;
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
@@ -226,20 +229,22 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
         if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
         if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
     };
-    long r = k.r0 + row;
-    for (; r + per_pass < k.r1; r += 2l * per_pass) {
-        typename Pack<T, V>::type vx[2], vd[2], vr[2];
+    walk<kGradTile, true>(sh, k.blk, row, per_pass,                    // last rows first, as in the forward
+        [&](long r) {
+            typename Pack<T, V>::type vx[kGradTile], vd[kGradTile], vr[kGradTile];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
-            vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
-            if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
-            else vr[u] = vx[u];
-        }
+            for (int u = 0; u < kGradTile; ++u) {
+                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
+                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+                else vr[u] = vx[u];
+            }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) one(r + (long)u * per_pass, vx[u], vd[u], vr[u]);
-    }
-    if (r < k.r1) one(r, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+            for (int u = 0; u < kGradTile; ++u) one(r + (long)u * per_pass, vx[u], vd[u], vr[u]);
+        },
+        [&](long r) {
+            one(r, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
+        });
 }
 
 // All rows of one chunk of one sample in registers, M vectors of x and of dy a thread.  direct: one sample, its channel sums are
@@ -342,7 +347,8 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     const T *dy = (const T*)f.dy, *x = (const T*)f.x, *res = (const T*)f.residual;
     T *dx = (T*)f.dx, *dres = (T*)f.dresidual;
     const bool params = f.dweight || f.dbias;
-    const unsigned param_blocks = params ? (unsigned)((sh.C + kParamCols - 1) / kParamCols) : 0;
+    // (a multiple of the eight dies, so that a row's workgroup stays on the die whose cache its sums were read into)
+    const unsigned param_blocks = params ? (unsigned)((sh.C + kParamCols - 1) / kParamCols + 7) / 8 * 8 : 0;
     const unsigned grid = (unsigned)((long)sh.N * sh.nblk * sh.chunks);
     if (p.threads) {
         const bool direct = sh.N == 1;
@@ -372,7 +378,7 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
         if (int rc = check_launch("msnet_group_norm_backward")) return rc;
     }
     Shape out = sh;
-    cut_rows(&out, V, kGradApplyBlocks, 4);
+    cut_rows(&out, V, kGradApplyBlocks, kGradTile, kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
     LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
     hipLaunchKernelGGL((group_norm_grad_apply<T, V, ACT, RES>), dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy,

@@ -646,36 +646,43 @@ def _is_dense(t):
     return True
 
 
-def _clip(grads, max_norm, outs):
-    """One msnet_clip_grads call over dense tensors (outs None: the norm alone)."""
-    from array import array
-    dev = torch.device("cuda", torch.cuda.current_device())
+def _clip(tables, count, max_norm, dev):
+    """One msnet_clip_grads call: tables as _host.tables returns them."""
+    src, dst, lengths, types, out_types = tables
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    pointers = lambda ts: array("Q", [t.data_ptr() for t in ts])                      # noqa: E731
-    types = lambda ts: bytes([_DTYPE_CODES[t.dtype] for t in ts])                     # noqa: E731
-    src, lengths, stypes = pointers(grads), array("q", [t.numel() for t in grads]), types(grads)
-    dst, dtypes = (src, stypes) if outs is grads else (pointers(outs), types(outs)) if outs is not None else (None, None)
-    addr = lambda a: a.buffer_info()[0] if a is not None else None                     # noqa: E731
     lib = _lib.load()
-    nbytes = lib.msnet_clip_grads_workspace_bytes(addr(lengths), len(grads))
-    ws = _workspace(nbytes, dev)
-    check(lib.msnet_clip_grads(addr(src), addr(dst), addr(lengths), stypes, dtypes, len(grads), max_norm, ptr(norm), ptr(ws), nbytes, stream_ptr()),
+    nbytes = lib.msnet_clip_grads_workspace_bytes(lengths, count)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    check(lib.msnet_clip_grads(src, dst or None, lengths, types, out_types or None, count, max_norm, ptr(norm), ptr(ws), nbytes, stream_ptr()),
           "msnet_clip_grads")
     return norm
 
 
-def _grad_list(grads, name):
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    for i, t in enumerate(grads):
-        _require_gpu(t, "%s[%d]" % (name, i))
-    return grads
+def _flat(t):
+    """A dense tensor's values in the order of its memory, as a contiguous tensor on that memory."""
+    return t.detach().as_strided((t.numel(),), (1,))
+
+
+def _grad_list(grads):
+    return [grads] if isinstance(grads, torch.Tensor) else list(grads)
+
+
+def _current_device():
+    return torch.device("cuda", torch.cuda.current_device())
 
 
 def grad_norm(grads):
     """The 2-norm over all values of all the given tensors (float32, float16, bfloat16, any shapes and mix): a float32 scalar on the
     device, nothing waits for it.  Squares are formed and added in 64 bits."""
-    grads = _grad_list(grads, "grads")
-    return _clip([t.detach() if _is_dense(t) else t.detach().contiguous() for t in grads], 0.0, None)
+    grads = _grad_list(grads)
+    host = _lib.load_host()
+    tables = host.tables(grads, None, torch.cuda.current_device()) if torch.cuda.is_available() else None
+    if tables is None:                                      # something to refuse, or to lay out
+        for i, t in enumerate(grads):
+            _require_gpu(t, "grads[%d]" % i)
+        grads = [_flat(t) if _is_dense(t) else t.detach().contiguous() for t in grads]
+        tables = host.tables(grads, None, torch.cuda.current_device())
+    return _clip(tables, len(grads), 0.0, _current_device())
 
 
 def clip_grads(grads, max_norm, out=None):
@@ -683,40 +690,49 @@ def clip_grads(grads, max_norm, out=None):
     in place, or into `out`, one tensor a gradient of its shape, of its type or float32.  Gradients that are short enough are left
     as they are (in place nothing is written).  The host is never asked: an infinite norm scales finite values to 0, and a NaN among
     the gradients makes all of them NaN.  A tensor listed twice, or one that overlaps another, is refused where it would be written."""
-    grads = _grad_list(grads, "grads")
+    grads = _grad_list(grads)
+    outs = grads if out is None else _grad_list(out)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative (got %r)" % (max_norm,))
-    if out is None:
-        outs = grads
+    host = _lib.load_host()
+    tables = host.tables(grads, outs, torch.cuda.current_device()) if torch.cuda.is_available() else None
+    if tables is not None:
+        norm = _clip(tables, len(grads), max_norm, _current_device())
     else:
-        outs = _grad_list(out, "out")
-        if len(outs) != len(grads):
-            raise ValueError("%d gradients, %d outputs" % (len(grads), len(outs)))
-        for i, (t, o) in enumerate(zip(grads, outs)):
-            if o.shape != t.shape or (o.dtype != t.dtype and o.dtype != torch.float32):
-                raise ValueError("out[%d] must be %s, %s or float32 (got %s %s)" % (i, tuple(t.shape), t.dtype, o.dtype, tuple(o.shape)))
-    if torch.is_grad_enabled() and any(o.requires_grad for o in outs):
-        raise ValueError("a tensor to be written requires a gradient itself")
-    src, dst, back = grads, outs, []
-    if not all(_is_dense(t) and _is_dense(o) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())) for t, o in zip(grads, outs)):
-        src, dst = [], []
-        for t, o in zip(grads, outs):                       # a value's place in memory has to be the same on both sides
-            same = t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())
-            if same and _is_dense(t):
-                src.append(t)
-                dst.append(o)
-            else:
-                if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-                    raise ValueError("a tensor to be written is expanded: its values share memory")
-                src.append(t.contiguous())
-                dst.append(torch.empty_like(src[-1], dtype=o.dtype))
-                back.append((o, dst[-1]))
-    norm = _clip(src, max_norm, src if dst is grads else dst)
-    for o, d in back:
-        o.copy_(d)
-    torch.autograd.graph.increment_version(outs)            # written behind autograd's back: what saved them finds out
+        src, dst, back = _clip_layout(grads, outs)
+        norm = _clip(host.tables(src, dst, torch.cuda.current_device()), len(src), max_norm, _current_device())
+        for o, d in back:
+            o.copy_(d)
+    host.written(outs)
     return norm
+
+
+def _clip_layout(grads, outs):
+    """What clip_grads refuses, and contiguous stand-ins for tensors of other layouts: (inputs, outputs, [(tensor, stand-in that holds
+    its new values)])."""
+    for name, ts in (("grads", grads), ("out", outs)):
+        for i, t in enumerate(ts):
+            _require_gpu(t, "%s[%d]" % (name, i))
+    if len(outs) != len(grads):
+        raise ValueError("%d gradients, %d outputs" % (len(grads), len(outs)))
+    src, dst, back = [], [], []
+    for i, (t, o) in enumerate(zip(grads, outs)):
+        if o.shape != t.shape or (o.dtype != t.dtype and o.dtype != torch.float32):
+            raise ValueError("out[%d] must be %s, %s or float32 (got %s %s)" % (i, tuple(t.shape), t.dtype, o.dtype, tuple(o.shape)))
+        if o.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a tensor to be written requires a gradient itself")
+        if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+            raise ValueError("a tensor to be written is expanded: its values share memory")
+        t, o = t.detach(), o.detach()
+        if _is_dense(t) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())):
+            src.append(_flat(t))                            # a value has the same place in memory on both sides
+            dst.append(_flat(o))
+        else:
+            src.append(t.contiguous().view(-1))
+            dst.append(torch.empty(src[-1].shape, device=o.device, dtype=o.dtype))
+            back.append((o, dst[-1].view(o.shape)))
+    return src, dst, back
 
 
 class _ActiveGuard(threading.local):
