@@ -79,7 +79,7 @@ struct Affine {
 // One row's V values: normalise, add the residual, activate, store; amax gathers magnitude bits for the range guard.
 template <class T, int V, int ACT>
 __device__ __forceinline__ void finish(const Affine<V>& k, const typename Pack<T, V>::type& x, const typename Pack<T, V>::type& res, bool has_res,
-                                       T* y, bool guard, unsigned& amax) {
+                                       T* y, bool stream, bool guard, unsigned& amax) {
     float o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -90,7 +90,7 @@ __device__ __forceinline__ void finish(const Affine<V>& k, const typename Pack<T
     if (guard)
 #pragma unroll
         for (int e = 0; e < V; ++e) amax = max(amax, __builtin_bit_cast(unsigned, o[e]) & 0x7fffffffu);
-    store<T, V>(y, o);
+    store<T, V>(y, o, stream);
 }
 
 // Per-thread sums into the workgroup's table: one column a vector where a vector lies in one group, one a channel elsewhere.
@@ -157,8 +157,9 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
                                                              const float* __restrict__ bias, const T* residual, Rows rr, T* y, Rows yr,
                                                              double2* __restrict__ stats, Shape sh, int slots,
                                                              const double2* __restrict__ part, const double* __restrict__ pivots,
-                                                             double m, double eps, unsigned* oflag) {
+                                                             double m, double eps, bool stream, unsigned* oflag) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics
+    const bool last = stream && !stats;                    // (a training step reads x and the residual again)
     double2* st = tab + kThreads;
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
@@ -181,20 +182,20 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
         [&](long r) {
             typename Pack<T, V>::type v[kTile], w[kTile];
 #pragma unroll
-            for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
+            for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss, last);
             if (residual)
 #pragma unroll
-                for (int u = 0; u < kTile; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+                for (int u = 0; u < kTile; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs, last);
             else
 #pragma unroll
                 for (int u = 0; u < kTile; ++u) w[u] = v[u];
 #pragma unroll
             for (int u = 0; u < kTile; ++u)
-                finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, oflag != nullptr, amax);
+                finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, stream, oflag != nullptr, amax);
         },
         [&](long r) {
             finish<T, V, ACT>(a, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pr + (size_t)r * rs), residual != nullptr, py + (size_t)r * yr.ss,
-                              oflag != nullptr, amax);
+                              stream, oflag != nullptr, amax);
         });
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);            // |y| >= 32752, inf or NaN: as the convs' epilogues
 }
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
         if (r < S) {
             auto w = v[i];
             if (residual) w = load_raw<T, V>(pr + (size_t)r * rr.ss);
-            finish<T, V, ACT>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
+            finish<T, V, ACT>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, false, oflag != nullptr, amax);
         }
     }
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);
@@ -354,7 +355,7 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     const long grid2 = (long)out.N * out.nblk * out.chunks;
     LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
     hipLaunchKernelGGL((group_norm_apply<T, V, ACT>), dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr,
-                       f.weight, f.bias, res, f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, m, f.eps, f.oflag);
+                       f.weight, f.bias, res, f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, m, f.eps, streams((double)sh.N * m * sh.G * sizeof(T)), f.oflag);
     return check_launch("msnet_group_norm");
 }
 

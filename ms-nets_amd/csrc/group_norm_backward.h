@@ -42,50 +42,58 @@ int backward_bf16(const Backward& f, const BackwardPlan& p, int act, void* ws);
 constexpr int kGradFew = 2;
 constexpr int grad_many(int V) { return V == 8 ? 4 : 8; }
 constexpr int kParamCols = 16;         // channels of one workgroup that sums dgamma and dbeta
-constexpr long kGradSumBlocks = 512, kGradApplyBlocks = 512;
-constexpr int kSumTile = 4, kGradTile = 2;             // rows a thread loads at once
+constexpr long kGradApplyBlocks = 512;
+constexpr long grad_sum_blocks(int V) { return V == 8 ? 512 : 768; }        // two or three of these fit a compute unit's registers
+// rows a thread loads at once (of eight channels the sums' registers leave room for two)
+constexpr int sum_tile(int V) { return V == 8 ? 2 : 4; }
+constexpr int kGradTile = 4;
 constexpr int kGradSumTiles = 2, kGradApplyTiles = 2;  // tiles of a workgroup at least
 
-// What a thread keeps of its V channels.
-template <int V>
+// What a thread keeps of its V channels.  WHOLE: they lie in one group, whose constants are kept once.
+template <int V, bool WHOLE>
 struct Channels {
-    float mean[V], rstd[V], lo[V], gamma[V], beta[V], near[V];
+    static constexpr int W = WHOLE ? 1 : V;
+    float mean[W], rstd[W], lo[W], gamma[V], beta[V];
     __device__ __forceinline__ void set(const double2* st, int c_local, int c, int cg, const float* weight, const float* bias) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
+        for (int e = 0; e < W; ++e) {
             const double2 t = st[(c_local + e) / cg];
             mean[e] = (float)t.x;
             rstd[e] = (float)t.y;
             lo[e] = (float)(((double)mean[e] - t.x) * t.y);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
             gamma[e] = weight ? weight[c + e] : 1.f;
             beta[e] = bias ? bias[c + e] : 0.f;
-            near[e] = gamma[e] == 0.f ? -1.f : 0x1p-20f * fabsf(lo[e] * gamma[e]);       // (gamma = 0: z is exact)
         }
     }
 };
 
 // dz and xhat of one row's V values.
-template <class T, int V, int ACT, bool RES>
-__device__ __forceinline__ void derive(const Channels<V>& k, const double2* st, int c_local, int cg, const typename Pack<T, V>::type& x,
+template <class T, int V, bool WHOLE, int ACT, bool RES>
+__device__ __forceinline__ void derive(const Channels<V, WHOLE>& k, const double2* st, int c_local, int cg, const typename Pack<T, V>::type& x,
                                        const typename Pack<T, V>::type& dy, const typename Pack<T, V>::type& res, float (&dz)[V], float (&xhat)[V]) {
     float z[V];
     bool near = false;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        xhat[e] = fmaf(element<T, V>(x, e) - k.mean[e], k.rstd[e], k.lo[e]);
+        const int g = WHOLE ? 0 : e;
+        xhat[e] = fmaf(element<T, V>(x, e) - k.mean[g], k.rstd[g], k.lo[g]);
         if constexpr (ACT != kNone) {
             const float b = RES ? k.beta[e] + element<T, V>(res, e) : k.beta[e];
             z[e] = fmaf(xhat[e], k.gamma[e], b);
-            if constexpr (ACT == kRelu) near |= fabsf(z[e]) <= fmaf(fabsf(b), 0x1p-20f, k.near[e]);
+            // (gamma = 0: z is exact, and often 0)
+            if constexpr (ACT == kRelu) near |= fabsf(z[e]) <= 0x1p-20f * (fabsf(b) + fabsf(k.lo[g] * k.gamma[e])) && k.gamma[e] != 0.f;
         }
     }
     if constexpr (ACT == kRelu)
         if (near)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                int c = c_local + e;                       // opaque to the compiler: it would form these doubles outside the loop over
-                float g = k.gamma[e], b = k.beta[e];       // the rows, for every thread, and spill registers to keep them
-                asm volatile("" : "+v"(c), "+v"(g), "+v"(b));
+                int c = c_local + e;                       // opaque to the compiler, and behind the element before: it would form
+                float g = k.gamma[e], b = k.beta[e];       // these doubles outside the loop over the rows and all V at once, for
+                asm volatile("" : "+v"(c), "+v"(g), "+v"(b), "+v"(z[e ? e - 1 : 0]));      // a branch hardly any row takes
                 const double2 t = st[c / cg];
                 double d = ((double)element<T, V>(x, e) - t.x) * t.y * (double)g + (double)b;
                 if constexpr (RES) d += (double)element<T, V>(res, e);
@@ -102,13 +110,14 @@ __device__ __forceinline__ void derive(const Channels<V>& k, const double2* st, 
     }
 }
 
-template <int V>
-__device__ __forceinline__ void grad_input(const Channels<V>& k, const float (&c1)[V], const float (&c2)[V], const float (&dz)[V],
-                                           const float (&xhat)[V], float (&dx)[V]) {
+template <int V, bool WHOLE>
+__device__ __forceinline__ void grad_input(const Channels<V, WHOLE>& k, const float (&c1)[WHOLE ? 1 : V], const float (&c2)[WHOLE ? 1 : V],
+                                           const float (&dz)[V], const float (&xhat)[V], float (&dx)[V]) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const float gz = k.gamma[e] * dz[e];       // (rounded before the subtraction: a group of one value has gz = c1 and dx = 0)
-        dx[e] = (__fsub_rn(gz, c1[e]) - xhat[e] * c2[e]) * k.rstd[e];
+        const int g = WHOLE ? 0 : e;
+        dx[e] = (__fsub_rn(gz, c1[g]) - xhat[e] * c2[g]) * k.rstd[g];
     }
 }
 
@@ -133,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_param_grads(const double2
     param_grads(chan, rows, C, blockIdx.x, dweight, dbias, tab);
 }
 
-template <class T, int V, int ACT, bool RES>
+template <class T, int V, bool WHOLE, int ACT, bool RES>
 __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
                                                                  const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                                  const float* __restrict__ bias, const double2* __restrict__ stats, Shape sh,
@@ -146,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
     for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
     __syncthreads();
     if (row < per_pass) {
-        Channels<V> a;
+        Channels<V, WHOLE> a;
         a.set(st, cl, k.c0 + cl, cg, weight, bias);
         double s[V], q[V];
 #pragma unroll
@@ -157,13 +166,14 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
         const long rs = RES ? rr.ss : xr.ss;
         auto add = [&](const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
             float dz[V], xhat[V];
-            derive<T, V, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
+            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 s[e] += (double)dz[e];
                 q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
             }
         };
+        constexpr int kSumTile = sum_tile(V);
         walk<kSumTile, false>(sh, k.blk, row, per_pass,
             [&](long r) {
                 typename Pack<T, V>::type vx[kSumTile], vd[kSumTile], vr[kSumTile];
@@ -192,13 +202,13 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
                [&](int g, double2 v) { part[slot * sh.G + k.g0 + g] = v; });
 }
 
-template <class T, int V, int ACT, bool RES>
+template <class T, int V, bool WHOLE, int ACT, bool RES>
 __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
                                                                   const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                                   const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
                                                                   T* __restrict__ dresidual, float* dweight, float* dbias, Shape sh, int slots,
                                                                   const double2* __restrict__ part, const double2* __restrict__ chan, long chan_rows,
-                                                                  int param_blocks, double m) {
+                                                                  int param_blocks, double m, bool stream) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics, [ng] c1 and c2
     if ((int)blockIdx.x < param_blocks) {
         param_grads(chan, chan_rows, sh.C, blockIdx.x, dweight, dbias, tab);
@@ -212,11 +222,11 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
     sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid,
               [&](int g, double2 sum) { coef[g] = make_double2(sum.x / m, sum.y / m); });
     if (row >= per_pass) return;
-    Channels<V> a;
+    Channels<V, WHOLE> a;
     a.set(st, cl, k.c0 + cl, cg, weight, bias);
-    float c1[V], c2[V];
+    float c1[WHOLE ? 1 : V], c2[WHOLE ? 1 : V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
+    for (int e = 0; e < (WHOLE ? 1 : V); ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
     const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
     const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
     const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
@@ -224,19 +234,19 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
     const size_t dense = (size_t)k.n * sh.S * sh.C + k.c0 + cl;
     auto one = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
         float dz[V], xhat[V], o[V];
-        derive<T, V, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
-        grad_input<V>(a, c1, c2, dz, xhat, o);
-        if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
-        if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
+        derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
+        grad_input<V, WHOLE>(a, c1, c2, dz, xhat, o);
+        if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o, stream);
+        if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz, stream);
     };
     walk<kGradTile, true>(sh, k.blk, row, per_pass,                    // last rows first, as in the forward
         [&](long r) {
             typename Pack<T, V>::type vx[kGradTile], vd[kGradTile], vr[kGradTile];
 #pragma unroll
             for (int u = 0; u < kGradTile; ++u) {
-                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
-                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
-                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
+                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss, stream);
+                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss, stream);
+                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs, stream);
                 else vr[u] = vx[u];
             }
 #pragma unroll
@@ -249,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
 
 // All rows of one chunk of one sample in registers, M vectors of x and of dy a thread.  direct: one sample, its channel sums are
 // dgamma and dbeta; else they go to chan[N][C].
-template <class T, int V, int M, int ACT, bool RES>
+template <class T, int V, bool WHOLE, int M, int ACT, bool RES>
 __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
                                                               const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                               const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
@@ -278,7 +288,7 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
             }
     }
     __syncthreads();
-    Channels<V> a;
+    Channels<V, WHOLE> a;
     double s[V], q[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
@@ -288,7 +298,7 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
         for (int i = 0; i < M; ++i)
             if (row + i * per_pass < S) {
                 float dz[V], xhat[V];
-                derive<T, V, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+                derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     s[e] += (double)dz[e];
@@ -321,17 +331,17 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
                [&](int g, double2 v) { coef[g] = make_double2(v.x / m, v.y / m); });
     __syncthreads();
     if (!on) return;
-    float c1[V], c2[V];
+    float c1[WHOLE ? 1 : V], c2[WHOLE ? 1 : V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
+    for (int e = 0; e < (WHOLE ? 1 : V); ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
     const size_t dense = (size_t)k.n * sh.S * sh.C + k.c0 + cl;
 #pragma unroll
     for (int i = 0; i < M; ++i) {
         const int r = row + i * per_pass;
         if (r < S) {
             float dz[V], xhat[V], o[V];
-            derive<T, V, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
-            grad_input<V>(a, c1, c2, dz, xhat, o);
+            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+            grad_input<V, WHOLE>(a, c1, c2, dz, xhat, o);
             if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
             if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
         }
@@ -340,7 +350,7 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 
-template <class T, int V, int ACT, bool RES>
+template <class T, int V, bool WHOLE, int ACT, bool RES>
 static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     const Shape& sh = p.shape;
     const double m = (double)sh.S * sh.cg, values = m * sh.N * sh.G;
@@ -357,10 +367,10 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
         {
             LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
             if (p.M == kGradFew)
-                hipLaunchKernelGGL((group_norm_grad_small<T, V, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
                                    f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
             else
-                hipLaunchKernelGGL((group_norm_grad_small<T, V, grad_many(V), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, grad_many(V), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
                                    f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
             if (int rc = check_launch("msnet_group_norm_backward")) return rc;
         }
@@ -373,7 +383,7 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     double2* chan = part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G;
     {
         LaunchScope ls("group_norm_grad_sums", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 3 : 2));
-        hipLaunchKernelGGL((group_norm_grad_sums<T, V, ACT, RES>), dim3(grid), dim3(kThreads), (kThreads * V + sh.gpc) * sizeof(double2), f.stream, dy,
+        hipLaunchKernelGGL((group_norm_grad_sums<T, V, WHOLE, ACT, RES>), dim3(grid), dim3(kThreads), (kThreads * V + sh.gpc) * sizeof(double2), f.stream, dy,
                            f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, sh, part, chan);
         if (int rc = check_launch("msnet_group_norm_backward")) return rc;
     }
@@ -381,24 +391,29 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     cut_rows(&out, V, kGradApplyBlocks, kGradTile, kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
     LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
-    hipLaunchKernelGGL((group_norm_grad_apply<T, V, ACT, RES>), dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy,
+    hipLaunchKernelGGL((group_norm_grad_apply<T, V, WHOLE, ACT, RES>), dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy,
                        f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, out, sh.nblk * sh.nsub, part, chan,
-                       (long)sh.N * sh.nblk, (int)param_blocks, m);
+                       (long)sh.N * sh.nblk, (int)param_blocks, m, streams(values * sizeof(T)));
     return check_launch("msnet_group_norm_backward");
+}
+
+template <class T, int V, bool WHOLE>
+static int backward_w(const Backward& f, const BackwardPlan& p, int act, void* ws) {
+    if (act == kRelu) return f.residual ? backward_act<T, V, WHOLE, kRelu, true>(f, p, ws) : backward_act<T, V, WHOLE, kRelu, false>(f, p, ws);
+    if (act == kSilu) return f.residual ? backward_act<T, V, WHOLE, kSilu, true>(f, p, ws) : backward_act<T, V, WHOLE, kSilu, false>(f, p, ws);
+    return backward_act<T, V, WHOLE, kNone, false>(f, p, ws);        // the residual's gradient is dy itself
 }
 
 template <class T, int V>
 static int backward_v(const Backward& f, const BackwardPlan& p, int act, void* ws) {
-    if (act == kRelu) return f.residual ? backward_act<T, V, kRelu, true>(f, p, ws) : backward_act<T, V, kRelu, false>(f, p, ws);
-    if (act == kSilu) return f.residual ? backward_act<T, V, kSilu, true>(f, p, ws) : backward_act<T, V, kSilu, false>(f, p, ws);
-    return backward_act<T, V, kNone, false>(f, p, ws);        // the residual's gradient is dy itself
+    return p.shape.cg % V == 0 ? backward_w<T, V, true>(f, p, act, ws) : backward_w<T, V, false>(f, p, act, ws);
 }
 
 template <class T>
 static int backward_t(const Backward& f, const BackwardPlan& p, int act, void* ws) {
     if constexpr (sizeof(T) == 2)
         if (p.V == 8) return backward_v<T, 8>(f, p, act, ws);
-    return p.V == 4 ? backward_v<T, 4>(f, p, act, ws) : backward_v<T, 1>(f, p, act, ws);
+    return p.V == 4 ? backward_v<T, 4>(f, p, act, ws) : backward_w<T, 1, true>(f, p, act, ws);
 }
 
 }  // namespace gn

@@ -33,7 +33,7 @@ BackwardPlan plan_backward(int N, long S, int C, int G, int dtype) {
     } else {
         p.V = vector_width(C, dtype);
         p.shape = make_shape(N, S, C, G, &p.V, (long)kThreads * p.V / 2);
-        cut_rows(&p.shape, p.V, kGradSumBlocks, kSumTile, kGradSumTiles);
+        cut_rows(&p.shape, p.V, grad_sum_blocks(p.V), sum_tile(p.V), kGradSumTiles);
         p.bytes = ((size_t)N * p.shape.nblk * p.shape.nsub * G + (size_t)N * p.shape.nblk * C) * sizeof(double2);
     }
     return p;
