@@ -125,16 +125,19 @@ def load():
 
 
 def load_host():
-    """The Python module _host (csrc/host_tables.cpp), loaded once; raises RuntimeError if it is not built."""
+    """The Python module _host (csrc/host_ops.cpp), loaded once and bound to the library; raises RuntimeError if it is not built."""
     global _host
     if _host is None:
-        import torch  # noqa: F401  (its libraries are what the module is linked against)
         import importlib
+        lib = load()                     # (imports torch first, whose libraries the module is linked against)
         try:
-            _host = importlib.import_module(__package__ + "._host")
+            host = importlib.import_module(__package__ + "._host")
         except ImportError as e:
             raise RuntimeError("ms-nets_amd/_host.so is not built or does not load (%s). Run `python -c 'import __graft_entry__ as g; "
                                "g.build()'`" % e) from e
+        host.bind({n: ctypes.cast(getattr(lib, n), c_void_p).value for n in SIGNATURES
+                   if n == "msnet_last_error" or n.startswith(("msnet_group_norm", "msnet_clip"))})
+        _host = host
     return _host
 
 

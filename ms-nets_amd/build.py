@@ -12,7 +12,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmsnet_hip.so")
-HOST = os.path.join(HERE, "_host.so")                 # Python module: reads lists of tensors (csrc/host_tables.cpp)
+HOST = os.path.join(HERE, "_host.so")                 # Python module: torch operators over the C ABI (csrc/host_ops.cpp)
 ARCH = "gfx950"
 
 # gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself.
@@ -154,17 +154,18 @@ def _build_locked(hipcc, objdir, out, force, verbose, defines):
 
 
 def build_host(force=False, verbose=True):
-    """The Python module _host (csrc/host_tables.cpp): host code against torch's headers, g++ alone."""
+    """The Python module _host (csrc/host_ops.cpp): host code against torch's headers, g++ alone."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension
-    src = os.path.join(CSRC, "host_tables.cpp")
+    src = os.path.join(CSRC, "host_ops.cpp")
     libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
-    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-    for inc in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]:
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    for inc in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]:
         flags += ["-isystem", inc]
-    links = ["-L" + libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
-    digest = _digest([src], flags + links + [torch.__version__, sys.version])
+    links = ["-L" + libdir, "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
+    digest = _digest([src, os.path.join(HERE, "..", "include", "msnet_hip.h")], flags + links + [torch.__version__, sys.version])
     if force or _stale(HOST, HOST + ".sha", digest):
         tmp = "%s.%d.tmp" % (HOST, os.getpid())
         cmd = ["g++"] + flags + [src, "-o", tmp] + links

@@ -20,14 +20,12 @@ enum DType { kF32 = 0, kF16 = 1, kBF16 = 2 };
 template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <class T> struct Pack<T, 1> { typedef T type; };
 
-template <class T, int V>
-__device__ __forceinline__ typename Pack<T, V>::type load_raw(const T* p) { return *reinterpret_cast<const typename Pack<T, V>::type*>(p); }
-
-// The same where `stream` says that nobody needs these values from the caches soon (streams(), below).
-template <class T, int V>
-__device__ __forceinline__ typename Pack<T, V>::type load_raw(const T* p, bool stream) {
+// STREAM: past the caches, which nobody needs these values from soon (streams(), below).
+template <class T, int V, bool STREAM = false>
+__device__ __forceinline__ typename Pack<T, V>::type load_raw(const T* p) {
     const auto q = reinterpret_cast<const typename Pack<T, V>::type*>(p);
-    return stream ? __builtin_nontemporal_load(q) : *q;
+    if constexpr (STREAM) return __builtin_nontemporal_load(q);
+    else return *q;
 }
 
 template <class T, int V>
@@ -36,15 +34,15 @@ __device__ __forceinline__ float element(const typename Pack<T, V>::type& r, int
     else return (float)r[e];
 }
 
-template <class T, int V>
-__device__ __forceinline__ void store(T* p, const float (&f)[V], bool stream = false) {
+template <class T, int V, bool STREAM = false>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
     typename Pack<T, V>::type o;
     if constexpr (V == 1) o = (T)f[0];
     else
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = (T)f[e];
     const auto q = reinterpret_cast<typename Pack<T, V>::type*>(p);
-    if (stream) __builtin_nontemporal_store(o, q);
+    if constexpr (STREAM) __builtin_nontemporal_store(o, q);
     else *q = o;
 }
 
@@ -56,7 +54,8 @@ struct Shape {
     int N, C, G, cg;                   // cg = C / G
     long S;
     int gpc, nsub, cw, chunks;
-    int nblk;                          // workgroups that share a sample's rows: tiles of kTile rows a thread, in turn (walk())
+    int nblk;                          // workgroups that share a sample's rows: tiles of a few rows a thread, in turn (Walk)
+    int rounds;                        // tiles of one of them, at most
 };
 
 struct Chunk {
@@ -81,21 +80,41 @@ __device__ __forceinline__ Chunk chunk_of(const Shape& s, unsigned b) {
 
 // The rows of one thread: the workgroups of a sample take tiles of U rows a thread in turn, so that all of them together stream
 // through one window of memory (each its own contiguous part instead made the finest level's passes 10 to 30 % slower: their
-// streams lie at like distances and meet in the same channels).  four(r) does rows r, r + step, .. r + (U - 1) step at once, one(r)
-// a single row; BACK starts at the last tile.
-template <int U, bool BACK, class Four, class One>
-__device__ __forceinline__ void walk(const Shape& s, int blk, int row, int step, Four four, One one) {
-    const long tile = (long)U * step, tiles = (s.S + tile - 1) / tile;
-    if (blk >= tiles) return;
-    const long rounds = (tiles - 1 - blk) / s.nblk + 1;
-    for (long i = 0; i < rounds; ++i) {
-        const long r = ((BACK ? rounds - 1 - i : i) * s.nblk + blk) * tile + row;
-        if (r + (long)(U - 1) * step < s.S) four(r);
-        else
-            for (int u = 0; u < U; ++u)
-                if (r + (long)u * step < s.S) one(r + (long)u * step);
+// streams lie at like distances and meet in the same channels).  BACK starts at the last tile.
+template <int U, bool BACK>
+struct Walk {
+    const Shape& s;
+    long row;
+    int blk, step;
+    bool on;
+    __device__ __forceinline__ Walk(const Shape& s_, int blk_, int row_, int step_, bool on_) : s(s_), row(row_), blk(blk_), step(step_), on(on_) {}
+    // tile(r) for whole tiles, one(r) for the rows of a tile that passes the end
+    template <class Whole, class One>
+    __device__ __forceinline__ void run(Whole tile, One one) const {
+        if (!on) return;
+        for (int i = 0; i < s.rounds; ++i) {
+            const long r = ((long)(BACK ? s.rounds - 1 - i : i) * s.nblk + blk) * (U * step) + row;
+            if (r + (long)(U - 1) * step < s.S) tile(r);
+            else
+                for (int u = 0; u < U; ++u)
+                    if (r + (long)u * step < s.S) one(r + (long)u * step);
+        }
     }
-}
+};
+
+// U rows of a thread's V channels, loaded at once.  A loads_issued() behind the tiles' loads keeps the compiler from moving them down
+// to their uses one by one, as it does for bf16 (sums of the finest level: 147 us with all in flight, 240 without).
+__device__ __forceinline__ void loads_issued() { __builtin_amdgcn_sched_barrier(0); }
+template <class T, int V, int U, bool STREAM = false>
+struct Tile {
+    typename Pack<T, V>::type v[U];
+    __device__ __forceinline__ void load(const T* p, long r, int step, long ss) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load_raw<T, V, STREAM>(p + (size_t)(r + (long)u * step) * ss);
+    }
+};
+
+__device__ __forceinline__ double2 shuffle_xor(double2 v, int o) { return make_double2(__shfl_xor(v.x, o), __shfl_xor(v.y, o)); }
 
 // Adds the rows of tab[rows][cols] into row 0, pairwise and in a fixed order; every thread of the workgroup takes part.
 __device__ __forceinline__ void sum_rows(double2* tab, int rows, int cols, int tid, int threads) {
@@ -109,7 +128,7 @@ __device__ __forceinline__ void sum_rows(double2* tab, int rows, int cols, int t
     __syncthreads();
 }
 
-// f(group, sum of its `per` consecutive columns of tab, each first put through w), called by one thread a group.
+// f(group, sum of its `per` consecutive entries of tab, each first put through w), called by one thread a group.
 template <class W, class F>
 __device__ __forceinline__ void sum_groups(const double2* tab, int per, int ng, int tid, int threads, W w, F f) {
     int lanes = 1;                     // threads of a group: a power of two, inside one wave
@@ -118,8 +137,33 @@ __device__ __forceinline__ void sum_groups(const double2* tab, int per, int ng, 
     for (int g = tid / lanes; g < ng; g += threads / lanes) {
         double2 s = make_double2(0., 0.);
         for (int i = lane; i < per; i += lanes) s = s + w(g * per + i, tab[g * per + i]);
-        for (int o = lanes >> 1; o > 0; o >>= 1) s = s + make_double2(__shfl_xor(s.x, o), __shfl_xor(s.y, o));
+        for (int o = lanes >> 1; o > 0; o >>= 1) s = s + shuffle_xor(s, o);
         if (lane == 0) f(g, s);
+    }
+}
+
+// Whether threads a power of two below a wave's width apart hold the same columns: their rows are added across the wave first.
+__device__ __forceinline__ bool in_wave(int columns) { return columns < 64 && (columns & (columns - 1)) == 0; }
+
+// Adds K values a thread over the rows (tid / cv) of threads with the same tid % cv: tab[(tid % cv) * K + j] gets the sums.  Every
+// thread takes part; `on` says whether it has a row.  tab: threads * K entries, or threads / 64 * cv * K where in_wave(cv).
+template <int K>
+__device__ __forceinline__ void sum_threads(double2 (&v)[K], double2* tab, int cv, bool on, int tid, int threads) {
+    if (in_wave(cv)) {
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            for (int o = cv; o < 64; o <<= 1) v[j] = v[j] + shuffle_xor(v[j], o);
+        if ((tid & 63) < cv) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) tab[((tid >> 6) * cv + (tid & 63)) * K + j] = v[j];
+        }
+        sum_rows(tab, threads >> 6, cv * K, tid, threads);
+    } else {
+        if (on) {
+#pragma unroll
+            for (int j = 0; j < K; ++j) tab[tid * K + j] = v[j];
+        }
+        sum_rows(tab, threads / cv, cv * K, tid, threads);
     }
 }
 
@@ -129,14 +173,13 @@ __device__ __forceinline__ void sum_slots(const double2* __restrict__ part, int 
     for (int gt = 0; gt < ng; gt += kThreads) {
         const int w = min(ng - gt, kThreads), lanes = kThreads / w;
         const int gi = tid % w, lane = tid / w;
+        double2 s[1] = {make_double2(0., 0.)};
         if (lane < lanes) {
-            double2 s = make_double2(0., 0.);
             const double2* p = part + g0 + gt + gi;
 #pragma unroll 4
-            for (int i = lane; i < slots; i += lanes) s = s + p[(size_t)i * G];
-            tab[tid] = s;
+            for (int i = lane; i < slots; i += lanes) s[0] = s[0] + p[(size_t)i * G];
         }
-        sum_rows(tab, lanes, w, tid, kThreads);
+        sum_threads<1>(s, tab, w, lane < lanes, tid, kThreads);
         if (tid < w) f(gt + tid, tab[tid]);
         __syncthreads();
     }
@@ -162,6 +205,9 @@ inline int vector_width(int C, int dtype) {
     const int full = 16 / element_bytes(dtype);
     return C % full == 0 ? full : C % 4 == 0 ? 4 : 1;
 }
+// In the single launches four at most: those wait for latencies, not for bandwidth, and eight channels' constants and sums do not
+// fit 1024 threads' registers.
+inline int small_vector_width(int C) { return C % 4 == 0 ? 4 : 1; }
 
 // Whether a result goes past the caches, and an input that is read for the last time too.  The last-level cache holds 256 MB: a
 // result of an eighth of it and more leaves there as a block of dirty lines that the next pass has to push out before it can keep
@@ -172,7 +218,7 @@ inline bool streams(double bytes) { return bytes >= 32e6; }
 int check_shape(const char* what, int dtype, int act, int N, long S, int C, int G, double eps);
 // V may be lowered to 1: groups whose edges fall inside vectors and that are too wide to be cut at a common multiple.
 Shape make_shape(int N, long S, int C, int G, int* V, long most_cw);
-// nblk: at most most_blocks workgroups in all, each at least `tiles` tiles of `tile` rows a thread.
+// nblk and rounds: at most most_blocks workgroups in all, each with `tiles` tiles of `tile` rows a thread or more.
 void cut_rows(Shape* s, int V, long most_blocks, int tile, int tiles);
 
 }  // namespace gn

@@ -8,6 +8,8 @@
 // Sums are of x - pivot and its square, in 64 bits (pivot: the group's first value): no cancellation for any mean, and the sign of
 // a value next to a ReLU's border comes out as in exact arithmetic, which the backward pass relies on.  gfx950 adds doubles at the
 // rate of floats, so the sums cost no more than three instructions a value.
+#include <type_traits>
+
 #include "group_norm.h"
 
 namespace msnet {
@@ -21,6 +23,8 @@ int check_shape(const char* what, int dtype, int act, int N, long S, int C, int 
     if (!(eps >= 0.)) return fail("%s: eps=%g", what, eps);
     return 0;
 }
+
+constexpr int kTile = 4;               // rows a thread loads at once
 
 static int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -45,17 +49,16 @@ Shape make_shape(int N, long S, int C, int G, int* V, long most_cw) {
 }
 
 void cut_rows(Shape* s, int V, long most_blocks, int tile, int tiles) {
-    const long least = (long)(kThreads / (s->cw / V)) * tile * tiles;
-    const long most = (s->S + least - 1) / least, nblk = most_blocks / ((long)s->N * s->chunks);
+    const long rows = (long)(kThreads / (s->cw / V)) * tile;           // of a tile (of the widest chunk: the last one's are longer)
+    const long all = (s->S + rows - 1) / rows, most = (all + tiles - 1) / tiles, nblk = most_blocks / ((long)s->N * s->chunks);
     s->nblk = (int)(nblk < 1 ? 1 : nblk < most ? nblk : most);
+    s->rounds = (int)((all + s->nblk - 1) / s->nblk);
 }
 
-constexpr int kTile = 4;               // rows a thread loads at once
-
-// mean and 1 / sqrt(var + eps) from the sums of x - pivot and of its square over m values
-__device__ __forceinline__ double2 statistics(double2 sum, double pivot, double m, double eps) {
-    const double d = sum.x / m;
-    double var = sum.y / m - d * d;
+// mean and 1 / sqrt(var + eps) from the sums of x - pivot and of its square; inv = 1 / m
+__device__ __forceinline__ double2 statistics(double2 sum, double pivot, double inv, double eps) {
+    const double d = sum.x * inv;
+    double var = sum.y * inv - d * d;
     var = var < 0. ? 0. : var;
     return make_double2(pivot + d, 1. / sqrt(var + eps));
 }
@@ -64,22 +67,31 @@ __device__ __forceinline__ double2 statistics(double2 sum, double pivot, double 
 template <int V>
 struct Affine {
     float mean[V], scale[V], shift[V];
-    __device__ __forceinline__ void set(const double2* st, int c_local, int c, int cg, const float* weight, const float* bias) {
+    // gamma and beta first, so that they arrive while the sums are formed
+    __device__ __forceinline__ void load(int c, const float* weight, const float* bias) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const double2 t = st[(c_local + e) / cg];
-            const double a = weight ? t.y * (double)weight[c + e] : t.y;
+            scale[e] = weight ? weight[c + e] : 1.f;
+            shift[e] = bias ? bias[c + e] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void set(const double2* st, int c_local, int cg, bool whole) {
+        double2 t = st[c_local / cg];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (!whole) t = st[(c_local + e) / cg];
+            const double a = t.y * (double)scale[e];
             mean[e] = (float)t.x;
             scale[e] = (float)a;
-            shift[e] = (float)((bias ? (double)bias[c + e] : 0.) - (t.x - (double)mean[e]) * a);
+            shift[e] = (float)((double)shift[e] - (t.x - (double)mean[e]) * a);
         }
     }
 };
 
 // One row's V values: normalise, add the residual, activate, store; amax gathers magnitude bits for the range guard.
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool STREAM>
 __device__ __forceinline__ void finish(const Affine<V>& k, const typename Pack<T, V>::type& x, const typename Pack<T, V>::type& res, bool has_res,
-                                       T* y, bool stream, bool guard, unsigned& amax) {
+                                       T* y, bool guard, unsigned& amax) {
     float o[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -90,22 +102,40 @@ __device__ __forceinline__ void finish(const Affine<V>& k, const typename Pack<T
     if (guard)
 #pragma unroll
         for (int e = 0; e < V; ++e) amax = max(amax, __builtin_bit_cast(unsigned, o[e]) & 0x7fffffffu);
-    store<T, V>(y, o, stream);
+    store<T, V, STREAM>(y, o);
 }
 
-// Per-thread sums into the workgroup's table: one column a vector where a vector lies in one group, one a channel elsewhere.
-template <int V>
-__device__ __forceinline__ void put_sums(double2* tab, int tid, bool whole, const double (&s)[V], const double (&q)[V]) {
-    if (whole) {
-        double a = s[0], b = q[0];
+// Sums of x - pivot and of its square, a channel.
+template <class T, int V>
+struct Sums {
+    double pivot[V], s[V], q[V];
+    __device__ __forceinline__ void start(const T (&first)[V]) {
 #pragma unroll
-        for (int e = 1; e < V; ++e) { a += s[e]; b += q[e]; }
-        tab[tid] = make_double2(a, b);
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) tab[tid * V + e] = make_double2(s[e], q[e]);
+        for (int e = 0; e < V; ++e) { pivot[e] = (double)(float)first[e]; s[e] = q[e] = 0.; }
     }
-}
+    __device__ __forceinline__ void add(const typename Pack<T, V>::type& v) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const double d = (double)element<T, V>(v, e) - pivot[e];
+            s[e] += d;
+            q[e] = fma(d, d, q[e]);
+        }
+    }
+    // Over the threads of a workgroup, into tab: one entry a vector where a vector lies in one group, one a channel elsewhere.
+    __device__ __forceinline__ void join(double2* tab, bool whole, int cv, bool on, int tid, int threads) {
+        if (whole) {
+            double2 v[1] = {make_double2(s[0], q[0])};
+#pragma unroll
+            for (int e = 1; e < V; ++e) { v[0].x += s[e]; v[0].y += q[e]; }
+            sum_threads<1>(v, tab, cv, on, tid, threads);
+        } else {
+            double2 v[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = make_double2(s[e], q[e]);
+            sum_threads<V>(v, tab, cv, on, tid, threads);
+        }
+    }
+};
 
 template <class T, int V>
 __global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict__ x, Rows xr, Shape sh, double2* __restrict__ part,
@@ -114,89 +144,79 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V;
-    const bool whole = sh.cg % V == 0;
+    const bool whole = sh.cg % V == 0, on = row < per_pass;
     const T* xn = x + (size_t)k.n * xr.sn;
-    double pivot[V], s[V], q[V];
+    const T* p = xn + k.c0 + cl;
+    T pivot[V];
+    pivot[0] = xn[(size_t)(k.g0 + (k.ng > 1 ? cl / sh.cg : 0)) * sh.cg];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        pivot[e] = (double)(float)xn[(size_t)(k.g0 + (k.ng > 1 ? (cl + e) / sh.cg : 0)) * sh.cg];
-        s[e] = q[e] = 0.;
-    }
+    for (int e = 1; e < V; ++e) pivot[e] = whole ? pivot[0] : xn[(size_t)(k.g0 + (k.ng > 1 ? (cl + e) / sh.cg : 0)) * sh.cg];
     if (k.blk == 0 && k.sub == 0)
         for (int g = tid; g < k.ng; g += kThreads) pivots[(size_t)k.n * sh.G + k.g0 + g] = (double)(float)xn[(size_t)(k.g0 + g) * sh.cg];
-    if (row < per_pass) {
-        const T* p = xn + k.c0 + cl;
-        auto add = [&](const typename Pack<T, V>::type& v) {
+    Sums<T, V> sums;
+    sums.start(pivot);
+    Walk<kTile, false>(sh, k.blk, row, per_pass, on).run(
+        [&](long r) {
+            Tile<T, V, kTile> t;
+            t.load(p, r, per_pass, xr.ss);
+            loads_issued();
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const double d = (double)element<T, V>(v, e) - pivot[e];
-                s[e] += d;
-                q[e] = fma(d, d, q[e]);
-            }
-        };
-        walk<kTile, false>(sh, k.blk, row, per_pass,
-            [&](long r) {
-                typename Pack<T, V>::type v[kTile];
-#pragma unroll
-                for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(p + (size_t)(r + (long)u * per_pass) * xr.ss);
-#pragma unroll
-                for (int u = 0; u < kTile; ++u) add(v[u]);
-            },
-            [&](long r) { add(load_raw<T, V>(p + (size_t)r * xr.ss)); });
-        put_sums<V>(tab, tid, whole, s, q);
-    }
-    const int cols = whole ? cv : k.cw;
-    sum_rows(tab, per_pass, cols, tid, kThreads);
+            for (int u = 0; u < kTile; ++u) sums.add(t.v[u]);
+        },
+        [&](long r) { sums.add(load_raw<T, V>(p + (size_t)r * xr.ss)); });
+    sums.join(tab, whole, cv, on, tid, kThreads);
     const size_t slot = (size_t)k.n * sh.nblk * sh.nsub + (size_t)k.blk * sh.nsub + k.sub;
-    sum_groups(tab, cols / k.ng, k.ng, tid, kThreads, [](int, double2 v) { return v; },
+    sum_groups(tab, (whole ? cv : k.cw) / k.ng, k.ng, tid, kThreads, [](int, double2 v) { return v; },
                [&](int g, double2 v) { part[slot * sh.G + k.g0 + g] = v; });
 }
 
-template <class T, int V, int ACT>
+// STREAM: y goes past the caches; without statistics to save (no backward will read them again) x and the residual do too.
+template <class T, int V, int ACT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr, const float* __restrict__ weight,
                                                              const float* __restrict__ bias, const T* residual, Rows rr, T* y, Rows yr,
                                                              double2* __restrict__ stats, Shape sh, int slots,
                                                              const double2* __restrict__ part, const double* __restrict__ pivots,
-                                                             double m, double eps, bool stream, unsigned* oflag) {
+                                                             double inv, double eps, unsigned* oflag) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics
-    const bool last = stream && !stats;                    // (a training step reads x and the residual again)
     double2* st = tab + kThreads;
+    const bool has_res = residual != nullptr;
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V;
+    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
+    const T* pr = has_res ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
+    const long rs = has_res ? rr.ss : xr.ss;
+    T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
+    Affine<V> a;
+    a.load(k.c0 + cl, weight, bias);
     sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid, [&](int g, double2 sum) {
         const size_t at = (size_t)k.n * sh.G + k.g0 + g;
-        const double2 t = statistics(sum, pivots[at], m, eps);
-        st[g] = t;
-        if (stats && k.blk == 0 && k.sub == 0) stats[at] = t;
+        const double2 v = statistics(sum, pivots[at], inv, eps);
+        st[g] = v;
+        if (stats && k.blk == 0 && k.sub == 0) stats[at] = v;
     });
-    if (row >= per_pass) return;
-    Affine<V> a;
-    a.set(st, cl, k.c0 + cl, k.ng > 1 ? sh.cg : k.cw, weight, bias);
-    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
-    const T* pr = residual ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
-    const long rs = residual ? rr.ss : xr.ss;
-    T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
+    a.set(st, cl, k.ng > 1 ? sh.cg : k.cw, sh.cg % V == 0);
     unsigned amax = 0u;
-    walk<kTile, true>(sh, k.blk, row, per_pass,                       // last rows first: what the sums read last is what the caches hold
-        [&](long r) {
-            typename Pack<T, V>::type v[kTile], w[kTile];
+    const auto put = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vr) {
+        finish<T, V, ACT, STREAM>(a, vx, vr, has_res, py + (size_t)r * yr.ss, oflag != nullptr, amax);
+    };
+    const auto rows = [&](auto last) {                     // last rows first: what the sums read last is what the caches hold
+        Walk<kTile, true>(sh, k.blk, row, per_pass, row < per_pass).run(
+            [&](long r) {
+                Tile<T, V, kTile, decltype(last)::value> x4, r4;
+                x4.load(px, r, per_pass, xr.ss);
+                if (has_res) r4.load(pr, r, per_pass, rs);
+                else r4 = x4;
+                loads_issued();
 #pragma unroll
-            for (int u = 0; u < kTile; ++u) v[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss, last);
-            if (residual)
-#pragma unroll
-                for (int u = 0; u < kTile; ++u) w[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs, last);
-            else
-#pragma unroll
-                for (int u = 0; u < kTile; ++u) w[u] = v[u];
-#pragma unroll
-            for (int u = 0; u < kTile; ++u)
-                finish<T, V, ACT>(a, v[u], w[u], residual != nullptr, py + (size_t)(r + (long)u * per_pass) * yr.ss, stream, oflag != nullptr, amax);
-        },
-        [&](long r) {
-            finish<T, V, ACT>(a, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pr + (size_t)r * rs), residual != nullptr, py + (size_t)r * yr.ss,
-                              stream, oflag != nullptr, amax);
-        });
+                for (int u = 0; u < kTile; ++u) put(r + (long)u * per_pass, x4.v[u], r4.v[u]);
+            },
+            [&](long r) { put(r, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pr + (size_t)r * rs)); });
+    };
+    if constexpr (STREAM) {
+        if (stats) rows(std::false_type{});
+        else rows(std::true_type{});
+    } else rows(std::false_type{});
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);            // |y| >= 32752, inf or NaN: as the convs' epilogues
 }
 
@@ -204,51 +224,40 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
 template <class T, int V, int M, int ACT>
 __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, const float* __restrict__ weight, const float* __restrict__ bias,
                                                          const T* residual, Rows rr, T* y, Rows yr, double2* __restrict__ stats, Shape sh,
-                                                         double m, double eps, unsigned* oflag) {
+                                                         double inv, double eps, unsigned* oflag) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
     const int row = tid / cv, cl = (tid % cv) * V;
-    const bool whole = sh.cg % V == 0;
-    const int cols = whole ? cv : k.cw;
+    const bool whole = sh.cg % V == 0, on = row < per_pass;
     double2* st = tab + (whole ? threads : threads * V);
     const T* xn = x + (size_t)k.n * xr.sn;
     const T* px = xn + k.c0 + cl;
     const int S = (int)sh.S;
+    T pivot[V];
+    pivot[0] = xn[(size_t)(k.g0 + cl / sh.cg) * sh.cg];
+#pragma unroll
+    for (int e = 1; e < V; ++e) pivot[e] = whole ? pivot[0] : xn[(size_t)(k.g0 + (cl + e) / sh.cg) * sh.cg];
     typename Pack<T, V>::type v[M];
-    if (row < per_pass) {
 #pragma unroll
-        for (int i = 0; i < M; ++i)
-            if (row + i * per_pass < S) v[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
-    }
-    double pivot[V], s[V], q[V];
+    for (int i = 0; i < M; ++i)
+        if (on && row + i * per_pass < S) v[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
+    Affine<V> a;
+    a.load(k.c0 + cl, weight, bias);
+    Sums<T, V> sums;
+    sums.start(pivot);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        pivot[e] = (double)(float)xn[(size_t)(k.g0 + (cl + e) / sh.cg) * sh.cg];
-        s[e] = q[e] = 0.;
-    }
-    if (row < per_pass) {
-#pragma unroll
-        for (int i = 0; i < M; ++i)
-            if (row + i * per_pass < S)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const double d = (double)element<T, V>(v[i], e) - pivot[e];
-                    s[e] += d;
-                    q[e] = fma(d, d, q[e]);
-                }
-        put_sums<V>(tab, tid, whole, s, q);
-    }
-    sum_rows(tab, per_pass, cols, tid, threads);
-    sum_groups(tab, cols / k.ng, k.ng, tid, threads, [](int, double2 u) { return u; }, [&](int g, double2 sum) {
-        const double2 t = statistics(sum, (double)(float)xn[(size_t)(k.g0 + g) * sh.cg], m, eps);
+    for (int i = 0; i < M; ++i)
+        if (on && row + i * per_pass < S) sums.add(v[i]);
+    sums.join(tab, whole, cv, on, tid, threads);
+    sum_groups(tab, (whole ? cv : k.cw) / k.ng, k.ng, tid, threads, [](int, double2 u) { return u; }, [&](int g, double2 sum) {
+        const double2 t = statistics(sum, (double)(float)xn[(size_t)(k.g0 + g) * sh.cg], inv, eps);
         st[g] = t;
         if (stats) stats[(size_t)k.n * sh.G + k.g0 + g] = t;
     });
     __syncthreads();                                       // statistics are there, and nobody reads x any more (y may be x)
-    if (row >= per_pass) return;
-    Affine<V> a;
-    a.set(st, cl, k.c0 + cl, sh.cg, weight, bias);
+    if (!on) return;
+    a.set(st, cl, sh.cg, whole);
     const T* pr = residual ? residual + (size_t)k.n * rr.sn + k.c0 + cl : nullptr;
     T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
     unsigned amax = 0u;
@@ -258,7 +267,7 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
         if (r < S) {
             auto w = v[i];
             if (residual) w = load_raw<T, V>(pr + (size_t)r * rr.ss);
-            finish<T, V, ACT>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, false, oflag != nullptr, amax);
+            finish<T, V, ACT, false>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
         }
     }
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);
@@ -313,7 +322,7 @@ struct Plan {
 
 static Plan plan_forward(int N, long S, int C, int G, int dtype) {
     Plan p = {};
-    p.V = vector_width(C, dtype);
+    p.V = small_vector_width(C);
     p.shape = small_shape(N, S, C, G, &p.V, dtype);
     p.threads = p.shape.nsub > 1 ? 0 : small_threads(p.shape, p.V, &p.M);
     if (!p.threads) {
@@ -332,17 +341,18 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     const T *x = (const T*)f.x, *res = (const T*)f.residual;
     const long grid = (long)sh.N * sh.nblk * sh.chunks;
     const size_t per_table = (sh.cg % V == 0 ? 1 : V) * sizeof(double2);
-    if (p.threads) {
-        const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
-        LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
-        if (p.M == 4)
-            hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias, res,
-                               f.rr, (T*)f.y, f.yr, f.stats, sh, m, f.eps, f.oflag);
-        else
-            hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias, res,
-                               f.rr, (T*)f.y, f.yr, f.stats, sh, m, f.eps, f.oflag);
-        return check_launch("msnet_group_norm");
-    }
+    if constexpr (V <= 4)
+        if (p.threads) {
+            const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
+            LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
+            if (p.M == 4)
+                hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                                   res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+            else
+                hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                                   res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+            return check_launch("msnet_group_norm");
+        }
     double2* part = (double2*)ws;
     double* pivots = (double*)(part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G);
     {
@@ -354,8 +364,9 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     cut_rows(&out, V, kApplyBlocks, kTile, kApplyTiles);
     const long grid2 = (long)out.N * out.nblk * out.chunks;
     LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
-    hipLaunchKernelGGL((group_norm_apply<T, V, ACT>), dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr,
-                       f.weight, f.bias, res, f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, m, f.eps, streams((double)sh.N * m * sh.G * sizeof(T)), f.oflag);
+    const auto apply = streams((double)sh.N * m * sh.G * sizeof(T)) ? group_norm_apply<T, V, ACT, true> : group_norm_apply<T, V, ACT, false>;
+    hipLaunchKernelGGL(apply, dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr, f.weight, f.bias, res,
+                       f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, 1. / m, f.eps, f.oflag);
     return check_launch("msnet_group_norm");
 }
 

@@ -40,7 +40,8 @@ int backward_bf16(const Backward& f, const BackwardPlan& p, int act, void* ws);
 
 // vectors of x and dy a thread of the single launch holds (1024 threads leave 128 registers each)
 constexpr int kGradFew = 2;
-constexpr int grad_many(int V) { return V == 8 ? 4 : 8; }
+constexpr int grad_many(int V, int bytes) { return V * bytes == 16 ? 4 : 8; }
+constexpr int kGradTable = 2048;       // sums of the single launch's threads at a time: 32 KB
 constexpr int kParamCols = 16;         // channels of one workgroup that sums dgamma and dbeta
 constexpr long kGradApplyBlocks = 512;
 constexpr long grad_sum_blocks(int V) { return V == 8 ? 512 : 768; }        // two or three of these fit a compute unit's registers
@@ -54,18 +55,20 @@ template <int V, bool WHOLE>
 struct Channels {
     static constexpr int W = WHOLE ? 1 : V;
     float mean[W], rstd[W], lo[W], gamma[V], beta[V];
-    __device__ __forceinline__ void set(const double2* st, int c_local, int c, int cg, const float* weight, const float* bias) {
+    __device__ __forceinline__ void load(int c, const float* weight, const float* bias) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            gamma[e] = weight ? weight[c + e] : 1.f;
+            beta[e] = bias ? bias[c + e] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void set(const double2* st, int c_local, int cg) {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
             const double2 t = st[(c_local + e) / cg];
             mean[e] = (float)t.x;
             rstd[e] = (float)t.y;
             lo[e] = (float)(((double)mean[e] - t.x) * t.y);
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            gamma[e] = weight ? weight[c + e] : 1.f;
-            beta[e] = bias ? bias[c + e] : 0.f;
         }
     }
 };
@@ -142,73 +145,81 @@ __global__ __launch_bounds__(kThreads) void group_norm_param_grads(const double2
     param_grads(chan, rows, C, blockIdx.x, dweight, dbias, tab);
 }
 
+// What a thread reads: x, dy and the residual at its channels of a sample; one row or a tile of them.
+template <class T, int V, bool RES>
+struct Inputs {
+    const T *x, *dy, *r;
+    long xs, ys, rs;
+    __device__ __forceinline__ Inputs(const T* x_, Rows xr, const T* dy_, Rows yr, const T* r_, Rows rr, int n, int c)
+        : x(x_ + (size_t)n * xr.sn + c), dy(dy_ + (size_t)n * yr.sn + c), r(RES ? r_ + (size_t)n * rr.sn + c : x), xs(xr.ss), ys(yr.ss), rs(RES ? rr.ss : xr.ss) {}
+    template <class F>
+    __device__ __forceinline__ void row(long at, F f) const {
+        f(at, load_raw<T, V>(x + (size_t)at * xs), load_raw<T, V>(dy + (size_t)at * ys), load_raw<T, V>(r + (size_t)at * rs));
+    }
+    template <int U, bool STREAM, class F>
+    __device__ __forceinline__ void tile(long at, int step, F f) const {
+        Tile<T, V, U, STREAM> tx, td, tr;
+        tx.load(x, at, step, xs);
+        td.load(dy, at, step, ys);
+        if constexpr (RES) tr.load(r, at, step, rs);
+        else tr = tx;
+        loads_issued();
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(at + (long)u * step, tx.v[u], td.v[u], tr.v[u]);
+    }
+};
+
 template <class T, int V, bool WHOLE, int ACT, bool RES>
 __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
                                                                  const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                                  const float* __restrict__ bias, const double2* __restrict__ stats, Shape sh,
                                                                  double2* __restrict__ part, double2* __restrict__ chan) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads * V] sums, [ng] statistics
+    constexpr int U = sum_tile(V);
     double2* st = tab + kThreads * V;
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
+    const bool on = row < per_pass;
     for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
+    Channels<V, WHOLE> a;
+    a.load(k.c0 + cl, weight, bias);
     __syncthreads();
-    if (row < per_pass) {
-        Channels<V, WHOLE> a;
-        a.set(st, cl, k.c0 + cl, cg, weight, bias);
-        double s[V], q[V];
+    a.set(st, cl, cg);
+    double s[V], q[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
-        const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
-        const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
-        const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
-        const long rs = RES ? rr.ss : xr.ss;
-        auto add = [&](const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
-            float dz[V], xhat[V];
-            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
+    for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
+    const auto add = [&](long, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
+        float dz[V], xhat[V];
+        derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                s[e] += (double)dz[e];
-                q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
-            }
-        };
-        constexpr int kSumTile = sum_tile(V);
-        walk<kSumTile, false>(sh, k.blk, row, per_pass,
-            [&](long r) {
-                typename Pack<T, V>::type vx[kSumTile], vd[kSumTile], vr[kSumTile];
+        for (int e = 0; e < V; ++e) {
+            s[e] += (double)dz[e];
+            q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
+        }
+    };
+    const Inputs<T, V, RES> in(x, xr, dy, yr, residual, rr, k.n, k.c0 + cl);
+    Walk<U, false>(sh, k.blk, row, per_pass, on).run([&](long r) { in.template tile<U, false>(r, per_pass, add); }, [&](long r) { in.row(r, add); });
+    double2 v[V];
 #pragma unroll
-                for (int u = 0; u < kSumTile; ++u) {
-                    vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss);
-                    vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss);
-                    if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs);
-                    else vr[u] = vx[u];
-                }
-#pragma unroll
-                for (int u = 0; u < kSumTile; ++u) add(vx[u], vd[u], vr[u]);
-            },
-            [&](long r) {
-                add(load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
-            });
-#pragma unroll
-        for (int e = 0; e < V; ++e) tab[tid * V + e] = make_double2(s[e], q[e]);
-    }
-    sum_rows(tab, per_pass, k.cw, tid, kThreads);
+    for (int e = 0; e < V; ++e) v[e] = make_double2(s[e], q[e]);
+    sum_threads<V>(v, tab, cv, on, tid, kThreads);
     double2* mine = chan + ((size_t)k.n * sh.nblk + k.blk) * sh.C + k.c0;
     for (int c = tid; c < k.cw; c += kThreads) mine[c] = tab[c];
     const size_t slot = (size_t)k.n * sh.nblk * sh.nsub + (size_t)k.blk * sh.nsub + k.sub;
     sum_groups(tab, k.cw / k.ng, k.ng, tid, kThreads,
-               [&](int c, double2 v) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * v.x, g * v.y); },
-               [&](int g, double2 v) { part[slot * sh.G + k.g0 + g] = v; });
+               [&](int c, double2 u) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * u.x, g * u.y); },
+               [&](int g, double2 u) { part[slot * sh.G + k.g0 + g] = u; });
 }
 
-template <class T, int V, bool WHOLE, int ACT, bool RES>
+// STREAM: the gradients go past the caches, and so do the inputs, read for the last time.
+template <class T, int V, bool WHOLE, int ACT, bool RES, bool STREAM>
 __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __restrict__ dy, Rows yr, const T* __restrict__ x, Rows xr,
                                                                   const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                                   const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
                                                                   T* __restrict__ dresidual, float* dweight, float* dbias, Shape sh, int slots,
                                                                   const double2* __restrict__ part, const double2* __restrict__ chan, long chan_rows,
-                                                                  int param_blocks, double m, bool stream) {
+                                                                  int param_blocks, double inv) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads] sums, [ng] statistics, [ng] c1 and c2
     if ((int)blockIdx.x < param_blocks) {
         param_grads(chan, chan_rows, sh.C, blockIdx.x, dweight, dbias, tab);
@@ -219,42 +230,25 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
     for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
-    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid,
-              [&](int g, double2 sum) { coef[g] = make_double2(sum.x / m, sum.y / m); });
-    if (row >= per_pass) return;
     Channels<V, WHOLE> a;
-    a.set(st, cl, k.c0 + cl, cg, weight, bias);
+    a.load(k.c0 + cl, weight, bias);
+    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid,
+              [&](int g, double2 sum) { coef[g] = make_double2(sum.x * inv, sum.y * inv); });
+    a.set(st, cl, cg);
     float c1[WHOLE ? 1 : V], c2[WHOLE ? 1 : V];
 #pragma unroll
     for (int e = 0; e < (WHOLE ? 1 : V); ++e) { c1[e] = (float)coef[(cl + e) / cg].x; c2[e] = (float)coef[(cl + e) / cg].y; }
-    const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
-    const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
-    const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
-    const long rs = RES ? rr.ss : xr.ss;
     const size_t dense = (size_t)k.n * sh.S * sh.C + k.c0 + cl;
-    auto one = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
+    const auto put = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vd, const typename Pack<T, V>::type& vr) {
         float dz[V], xhat[V], o[V];
         derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx, vd, vr, dz, xhat);
         grad_input<V, WHOLE>(a, c1, c2, dz, xhat, o);
-        if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o, stream);
-        if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz, stream);
+        if (dx) store<T, V, STREAM>(dx + dense + (size_t)r * sh.C, o);
+        if (RES && dresidual) store<T, V, STREAM>(dresidual + dense + (size_t)r * sh.C, dz);
     };
-    walk<kGradTile, true>(sh, k.blk, row, per_pass,                    // last rows first, as in the forward
-        [&](long r) {
-            typename Pack<T, V>::type vx[kGradTile], vd[kGradTile], vr[kGradTile];
-#pragma unroll
-            for (int u = 0; u < kGradTile; ++u) {
-                vx[u] = load_raw<T, V>(px + (size_t)(r + (long)u * per_pass) * xr.ss, stream);
-                vd[u] = load_raw<T, V>(pd + (size_t)(r + (long)u * per_pass) * yr.ss, stream);
-                if constexpr (RES) vr[u] = load_raw<T, V>(pr + (size_t)(r + (long)u * per_pass) * rs, stream);
-                else vr[u] = vx[u];
-            }
-#pragma unroll
-            for (int u = 0; u < kGradTile; ++u) one(r + (long)u * per_pass, vx[u], vd[u], vr[u]);
-        },
-        [&](long r) {
-            one(r, load_raw<T, V>(px + (size_t)r * xr.ss), load_raw<T, V>(pd + (size_t)r * yr.ss), load_raw<T, V>(pr + (size_t)r * rs));
-        });
+    const Inputs<T, V, RES> in(x, xr, dy, yr, residual, rr, k.n, k.c0 + cl);
+    Walk<kGradTile, true>(sh, k.blk, row, per_pass, row < per_pass).run(             // last rows first, as in the forward
+        [&](long r) { in.template tile<kGradTile, STREAM>(r, per_pass, put); }, [&](long r) { in.row(r, put); });
 }
 
 // All rows of one chunk of one sample in registers, M vectors of x and of dy a thread.  direct: one sample, its channel sums are
@@ -264,10 +258,10 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
                                                               const T* __restrict__ residual, Rows rr, const float* __restrict__ weight,
                                                               const float* __restrict__ bias, const double2* __restrict__ stats, T* __restrict__ dx,
                                                               T* __restrict__ dresidual, float* dweight, float* dbias, Shape sh,
-                                                              double2* __restrict__ chan, bool direct, double m) {
-    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [2048] sums of a round, [cw] of the channels, [ng] statistics
+                                                              double2* __restrict__ chan, bool direct, double inv) {
+    extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kGradTable] sums, [cw] of the channels, [ng] statistics, [ng] c1 and c2
     const Chunk k = chunk_of(sh, blockIdx.x);
-    double2 *sums = tab + 2048, *st = sums + k.cw, *coef = tab;
+    double2 *st = tab + kGradTable + k.cw, *coef = st + k.ng;
     const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = sh.cg;
     const int S = (int)sh.S;
@@ -287,38 +281,36 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
                 else vr[i] = vx[i];
             }
     }
-    __syncthreads();
     Channels<V, WHOLE> a;
-    double s[V], q[V];
+    a.load(k.c0 + cl, weight, bias);
+    __syncthreads();
+    a.set(st, cl, cg);
+    double2 v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = q[e] = 0.;
-    if (on) {
-        a.set(st, cl, k.c0 + cl, cg, weight, bias);
+    for (int e = 0; e < V; ++e) v[e] = make_double2(0., 0.);
 #pragma unroll
-        for (int i = 0; i < M; ++i)
-            if (row + i * per_pass < S) {
-                float dz[V], xhat[V];
-                derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+    for (int i = 0; i < M; ++i)
+        if (on && row + i * per_pass < S) {
+            float dz[V], xhat[V];
+            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    s[e] += (double)dz[e];
-                    q[e] = fma((double)dz[e], (double)xhat[e], q[e]);
-                }
+            for (int e = 0; e < V; ++e) {
+                v[e].x += (double)dz[e];
+                v[e].y = fma((double)dz[e], (double)xhat[e], v[e].y);
             }
-    }
-    // channel sums, at most 2048 of the threads' values in the table at a time
-    const int round = min(V, 2048 / threads);
-#pragma unroll
-    for (int e0 = 0; e0 < V; ++e0) {
-        if (e0 % round) continue;
-        if (on) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (e >= e0 && e < e0 + round) tab[(row * cv + cl / V) * round + e - e0] = make_double2(s[e], q[e]);
         }
-        sum_rows(tab, per_pass, cv * round, tid, threads);
-        for (int i = tid; i < cv * round; i += threads) sums[i / round * V + e0 + i % round] = tab[i];
-        __syncthreads();
+    double2* sums = tab;                                   // of the channels
+    if (threads * V <= kGradTable || (in_wave(cv) && (threads >> 6) * k.cw <= kGradTable)) {
+        sum_threads<V>(v, tab, cv, on, tid, threads);
+    } else {                                               // an element of all vectors at a time, each round's sums put behind the table
+        sums = tab + kGradTable;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            double2 u[1] = {v[e]};
+            sum_threads<1>(u, tab, cv, on, tid, threads);
+            for (int i = tid; i < cv; i += threads) sums[i * V + e] = tab[i];
+            __syncthreads();
+        }
     }
     for (int c = tid; c < k.cw; c += threads) {
         if (direct) {
@@ -327,8 +319,8 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
         } else if (chan) chan[(size_t)k.n * sh.C + k.c0 + c] = sums[c];
     }
     sum_groups(sums, cg, k.ng, tid, threads,
-               [&](int c, double2 v) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * v.x, g * v.y); },
-               [&](int g, double2 v) { coef[g] = make_double2(v.x / m, v.y / m); });
+               [&](int c, double2 u) { const double g = weight ? (double)weight[k.c0 + c] : 1.; return make_double2(g * u.x, g * u.y); },
+               [&](int g, double2 u) { coef[g] = make_double2(u.x * inv, u.y * inv); });
     __syncthreads();
     if (!on) return;
     float c1[WHOLE ? 1 : V], c2[WHOLE ? 1 : V];
@@ -360,25 +352,26 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     // (a multiple of the eight dies, so that a row's workgroup stays on the die whose cache its sums were read into)
     const unsigned param_blocks = params ? (unsigned)((sh.C + kParamCols - 1) / kParamCols + 7) / 8 * 8 : 0;
     const unsigned grid = (unsigned)((long)sh.N * sh.nblk * sh.chunks);
-    if (p.threads) {
-        const bool direct = sh.N == 1;
-        double2* chan = direct || !params ? nullptr : (double2*)ws;
-        const size_t lds = (2048 + sh.cw + sh.gpc) * sizeof(double2);
-        {
-            LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
-            if (p.M == kGradFew)
-                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
-                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
-            else
-                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, grad_many(V), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
-                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, m);
-            if (int rc = check_launch("msnet_group_norm_backward")) return rc;
+    if constexpr (V <= 4)
+        if (p.threads) {
+            const bool direct = sh.N == 1;
+            double2* chan = direct || !params ? nullptr : (double2*)ws;
+            const size_t lds = (kGradTable + sh.cw + 2 * sh.gpc) * sizeof(double2);
+            {
+                LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
+                if (p.M == kGradFew)
+                    hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                       f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
+                else
+                    hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, grad_many(V, sizeof(T)), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                       f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
+                if (int rc = check_launch("msnet_group_norm_backward")) return rc;
+            }
+            if (!chan) return 0;
+            LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.C);
+            hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N, sh.C, f.dweight, f.dbias);
+            return check_launch("msnet_group_norm_backward");
         }
-        if (!chan) return 0;
-        LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.C);
-        hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N, sh.C, f.dweight, f.dbias);
-        return check_launch("msnet_group_norm_backward");
-    }
     double2* part = (double2*)ws;
     double2* chan = part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G;
     {
@@ -391,9 +384,9 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     cut_rows(&out, V, kGradApplyBlocks, kGradTile, kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
     LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
-    hipLaunchKernelGGL((group_norm_grad_apply<T, V, WHOLE, ACT, RES>), dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy,
-                       f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, out, sh.nblk * sh.nsub, part, chan,
-                       (long)sh.N * sh.nblk, (int)param_blocks, m, streams(values * sizeof(T)));
+    const auto apply = streams(values * sizeof(T)) ? group_norm_grad_apply<T, V, WHOLE, ACT, RES, true> : group_norm_grad_apply<T, V, WHOLE, ACT, RES, false>;
+    hipLaunchKernelGGL(apply, dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy, f.yr, x, f.xr, res, f.rr, f.weight,
+                       f.bias, f.stats, dx, dres, f.dweight, f.dbias, out, sh.nblk * sh.nsub, part, chan, (long)sh.N * sh.nblk, (int)param_blocks, 1. / m);
     return check_launch("msnet_group_norm_backward");
 }
 

@@ -6,10 +6,10 @@ namespace gn {
 
 int backward_f32(const Backward& f, const BackwardPlan& p, int act, void* ws) { return backward_t<float>(f, p, act, ws); }
 
-static int grad_small_threads(const Shape& s, int V, int* M) {
+static int grad_small_threads(const Shape& s, int V, int dtype, int* M) {
     const int cv = s.cw / V;
-    if ((2048 + s.cw + s.gpc) * sizeof(double2) > 65536) return 0;
-    for (int m : {kGradFew, grad_many(V)})
+    if ((kGradTable + s.cw + 2 * s.gpc) * sizeof(double2) > 65536) return 0;
+    for (int m : {kGradFew, grad_many(V, element_bytes(dtype))})
         for (int t = 256; t <= 1024; t <<= 1)
             if (s.S <= (long)m * (t / cv)) { *M = m; return t; }
     return 0;
@@ -18,16 +18,16 @@ static int grad_small_threads(const Shape& s, int V, int* M) {
 BackwardPlan plan_backward(int N, long S, int C, int G, int dtype) {
     BackwardPlan p = {};
     long w = 64 / element_bytes(dtype);                     // 64-byte row segments, wider ones once workgroups abound (as in the forward)
-    p.V = vector_width(C, dtype);
+    p.V = small_vector_width(C);
     p.shape = make_shape(N, S, C, G, &p.V, w);
     while ((long)N * p.shape.chunks > 2048 && w < (long)kThreads * p.V) {
         w *= 2;
         int M;
         const Shape t = make_shape(N, S, C, G, &p.V, w);
-        if (t.nsub > 1 || !grad_small_threads(t, p.V, &M)) break;
+        if (t.nsub > 1 || !grad_small_threads(t, p.V, dtype, &M)) break;
         p.shape = t;
     }
-    p.threads = p.shape.nsub > 1 ? 0 : grad_small_threads(p.shape, p.V, &p.M);
+    p.threads = p.shape.nsub > 1 ? 0 : grad_small_threads(p.shape, p.V, dtype, &p.M);
     if (p.threads) {
         p.bytes = N > 1 ? (size_t)N * C * sizeof(double2) : 0;
     } else {

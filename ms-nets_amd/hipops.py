@@ -485,15 +485,6 @@ def _row_strides(t):
     return (st[0], 0 if row is None else row)
 
 
-def _rows(t):
-    """t as the kernels read it, and its strides: itself, or a contiguous copy."""
-    strides = _row_strides(t)
-    if strides is None:
-        t = t.contiguous()
-        strides = _row_strides(t)
-    return t, strides
-
-
 def _extent(t):
     """[first byte, behind the last byte) of a tensor's values."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
@@ -537,61 +528,6 @@ def _check_norm_args(x, groups, weight, bias, eps, act, residual):
             raise ValueError("residual %s %s differs from x %s %s" % (residual.dtype, tuple(residual.shape), x.dtype, tuple(x.shape)))
 
 
-def _norm_dims(x, groups):
-    n, c = x.shape[0], x.shape[-1]
-    return n, (x.numel() // (n * c) if n else 0), c, int(groups)
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
-
-
-def _group_norm_forward(x, groups, weight, bias, eps, act, residual, y, stats, workspace=_workspace):
-    """One msnet_group_norm call into y; x and residual as _rows gives them."""
-    n, s, c, g = _norm_dims(x, groups)
-    lib, code, xs, ys = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(y)
-    rs = _row_strides(residual) if residual is not None else (0, 0)
-    nbytes = lib.msnet_group_norm_workspace_bytes(code, n, s, c, g)
-    ws = workspace(nbytes, x.device)
-    check(lib.msnet_group_norm(ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y), ptr(stats), code, _ACT_CODES[act], n, s, c, g, eps,
-                               xs[0], xs[1], rs[0], rs[1], ys[0], ys[1], ptr(ws), nbytes, stream_ptr()), "msnet_group_norm")
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, groups, eps, act):
-        x, _ = _rows(x)
-        if residual is not None:
-            residual, _ = _rows(residual)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        stats = torch.empty((x.shape[0], groups, 2), device=x.device, dtype=torch.float64)
-        _group_norm_forward(x, groups, weight, bias, eps, act, residual, y, stats)
-        ctx.groups, ctx.act = groups, act
-        ctx.save_for_backward(x, weight, bias, residual if act != "none" else None, stats)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, residual, stats = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dy, ds = _rows(dy)
-        xs = _row_strides(x)
-        rs = _row_strides(residual) if residual is not None else (0, 0)
-        n, s, c, g = _norm_dims(x, ctx.groups)
-        new = lambda wanted, shape, dtype: torch.empty(shape, device=x.device, dtype=dtype) if wanted else None      # noqa: E731
-        dx = new(need_x, x.shape, x.dtype)
-        dres = new(need_r and ctx.act != "none", x.shape, x.dtype)
-        dw, db = new(need_w, (c,), torch.float32), new(need_b, (c,), torch.float32)
-        lib, code = _lib.load(), _DTYPE_CODES[x.dtype]
-        nbytes = lib.msnet_group_norm_backward_workspace_bytes(code, n, s, c, g)
-        ws = _workspace(nbytes, x.device)
-        check(lib.msnet_group_norm_backward(ptr(dy), ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(stats), ptr(dx), ptr(dres), ptr(dw), ptr(db),
-                                            code, _ACT_CODES[ctx.act], n, s, c, g, ds[0], ds[1], xs[0], xs[1], rs[0], rs[1], ptr(ws), nbytes,
-                                            stream_ptr()), "msnet_group_norm_backward")
-        return dx, dw, db, (dy if need_r and ctx.act == "none" else dres), None, None, None
-
-
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual=None, out=None):
     """act(group_norm(x) * weight + bias (+ residual)) over a channels-last x [N, ..., C] (NDHWC activations, or [N, rows, C]):
     mean and variance over all positions and the C / groups channels of one sample and group.  x, residual and the result are
@@ -602,33 +538,39 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
     With gradients enabled the result is differentiable once in x, weight, bias and residual; x, the residual (with an activation)
     and 16 bytes a sample and group are kept for it.  Results and gradients repeat bit for bit.  Inside a forward of the aggregators
     the result raises the fp16-range flag as a conv's does (RangeGuard)."""
-    _check_norm_args(x, groups, weight, bias, eps, act, residual)
+    if out is None and _tls.arena is None and act in _ACT_CODES and type(groups) is int:
+        y = _lib.load_host().group_norm(x, groups, weight, bias, eps, _ACT_CODES[act], residual)
+        if y is not None:
+            return y
+    _check_norm_args(x, groups, weight, bias, eps, act, residual)       # something to refuse, to lay out or to place
     groups, eps = int(groups), float(eps)
-    if weight is not None and (weight.dtype != torch.float32 or not weight.is_contiguous()):
-        weight = weight.float().contiguous()
-    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
-        bias = bias.float().contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        if out is not None:
-            raise ValueError("out cannot be used where a gradient is asked for")
-        return _GroupNorm.apply(x, weight, bias, residual, groups, eps, act)
-    x, _ = _rows(x)
-    if residual is not None:
-        residual, _ = _rows(residual)
-    arena = _tls.arena is not None and x.dtype == torch.float32
+    plain = lambda p: p if p is None or (p.dtype == torch.float32 and p.is_contiguous()) else p.float().contiguous()      # noqa: E731
+    even = lambda t: t if t is None or _row_strides(t) is not None else t.contiguous()                                    # noqa: E731
+    x, residual, weight, bias = even(x), even(residual), plain(weight), plain(bias)
+    graded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
+    if graded and out is not None:
+        raise ValueError("out cannot be used where a gradient is asked for")
+    if out is None and (graded or _tls.arena is None or x.dtype != torch.float32):
+        y = _lib.load_host().group_norm(x, groups, weight, bias, eps, _ACT_CODES[act], residual)
+        assert y is not None
+        return y
+    n, s, c = x.shape[0], (x.numel() // (x.shape[0] * x.shape[-1]) if x.numel() else 0), x.shape[-1]
     if out is None:
-        out = _new(x.shape, x.device) if arena else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = _new(x.shape, x.device)
     else:
         _require_gpu(out, "out")
-        strides, (n, s, c, _) = _row_strides(out), _norm_dims(x, groups)
+        strides = _row_strides(out)
         if out.shape != x.shape or out.dtype != x.dtype or strides is None or (s > 1 and strides[1] < c) or (n > 1 and strides[0] < (s - 1) * strides[1] + c):
             raise ValueError("out must be %s %s with consecutive channels and evenly spaced rows of its own" % (x.dtype, tuple(x.shape)))
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("out must not require a gradient")
         _check_out(out, x, "x")
         _check_out(out, residual, "residual")
-    _group_norm_forward(x, groups, weight, bias, eps, act, residual, out, None,
-                        (lambda nbytes, dev: _new(((nbytes + 3) // 4,), dev) if nbytes else None) if arena else _workspace)
+    lib, code, xs, ys, rs = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(out), _row_strides(residual) if residual is not None else (0, 0)
+    nbytes = lib.msnet_group_norm_workspace_bytes(code, n, s, c, groups)
+    ws = None if not nbytes else _new(((nbytes + 3) // 4,), x.device) if _tls.arena is not None else torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    check(lib.msnet_group_norm(ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(out), None, code, _ACT_CODES[act], n, s, c, groups, eps, *xs, *rs, *ys,
+                               ptr(ws), nbytes, stream_ptr()), "msnet_group_norm")
     return out
 
 
@@ -646,18 +588,6 @@ def _is_dense(t):
     return True
 
 
-def _clip(tables, count, max_norm, dev):
-    """One msnet_clip_grads call: tables as _host.tables returns them."""
-    src, dst, lengths, types, out_types = tables
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    lib = _lib.load()
-    nbytes = lib.msnet_clip_grads_workspace_bytes(lengths, count)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    check(lib.msnet_clip_grads(src, dst or None, lengths, types, out_types or None, count, max_norm, ptr(norm), ptr(ws), nbytes, stream_ptr()),
-          "msnet_clip_grads")
-    return norm
-
-
 def _flat(t):
     """A dense tensor's values in the order of its memory, as a contiguous tensor on that memory."""
     return t.detach().as_strided((t.numel(),), (1,))
@@ -667,22 +597,17 @@ def _grad_list(grads):
     return [grads] if isinstance(grads, torch.Tensor) else list(grads)
 
 
-def _current_device():
-    return torch.device("cuda", torch.cuda.current_device())
-
-
 def grad_norm(grads):
     """The 2-norm over all values of all the given tensors (float32, float16, bfloat16, any shapes and mix): a float32 scalar on the
     device, nothing waits for it.  Squares are formed and added in 64 bits."""
     grads = _grad_list(grads)
     host = _lib.load_host()
-    tables = host.tables(grads, None, torch.cuda.current_device()) if torch.cuda.is_available() else None
-    if tables is None:                                      # something to refuse, or to lay out
+    norm = host.clip(grads, None, 0.0)
+    if norm is None:                                        # something to refuse, or to lay out
         for i, t in enumerate(grads):
             _require_gpu(t, "grads[%d]" % i)
-        grads = [_flat(t) if _is_dense(t) else t.detach().contiguous() for t in grads]
-        tables = host.tables(grads, None, torch.cuda.current_device())
-    return _clip(tables, len(grads), 0.0, _current_device())
+        norm = host.clip([_flat(t) if _is_dense(t) else t.detach().contiguous() for t in grads], None, 0.0)
+    return norm
 
 
 def clip_grads(grads, max_norm, out=None):
@@ -696,15 +621,13 @@ def clip_grads(grads, max_norm, out=None):
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative (got %r)" % (max_norm,))
     host = _lib.load_host()
-    tables = host.tables(grads, outs, torch.cuda.current_device()) if torch.cuda.is_available() else None
-    if tables is not None:
-        norm = _clip(tables, len(grads), max_norm, _current_device())
-    else:
+    norm = host.clip(grads, outs, max_norm)
+    if norm is None:
         src, dst, back = _clip_layout(grads, outs)
-        norm = _clip(host.tables(src, dst, torch.cuda.current_device()), len(src), max_norm, _current_device())
+        norm = host.clip(src, dst, max_norm)
         for o, d in back:
             o.copy_(d)
-    host.written(outs)
+        torch.autograd.graph.increment_version(outs)
     return norm
 
 
