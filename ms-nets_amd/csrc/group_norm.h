@@ -199,15 +199,11 @@ __device__ __forceinline__ float activate(float z) {
 // ---- host ------------------------------------------------------------------------------------------------------------
 inline int element_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
-// Channels a thread takes at once: 16 bytes of them where the channel count allows, 8 bytes for 16-bit types whose count is only a
-// multiple of four (C = 60: 8-byte lanes), single ones otherwise.
-inline int vector_width(int C, int dtype) {
-    const int full = 16 / element_bytes(dtype);
-    return C % full == 0 ? full : C % 4 == 0 ? 4 : 1;
-}
-// In the single launches four at most: those wait for latencies, not for bandwidth, and eight channels' constants and sums do not
-// fit 1024 threads' registers.
-inline int small_vector_width(int C) { return C % 4 == 0 ? 4 : 1; }
+// Channels a thread takes at once.  Four of any type: eight 16-bit ones (16-byte lanes, groups of four or fewer inside a vector) were
+// no faster on any size once eight rows of four are loaded at once, and 5 us slower on the smallest.
+inline int vector_width(int C) { return C % 4 == 0 ? 4 : C % 2 == 0 ? 2 : 1; }
+// Rows of a thread's vectors that are loaded at once where bandwidth decides.
+constexpr int tile_rows(int V, int bytes) { return V * bytes == 16 ? 4 : 8; }
 
 // Whether a result goes past the caches, and an input that is read for the last time too.  The last-level cache holds 256 MB: a
 // result of an eighth of it and more leaves there as a block of dirty lines that the next pass has to push out before it can keep

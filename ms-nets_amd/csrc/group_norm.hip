@@ -24,8 +24,6 @@ int check_shape(const char* what, int dtype, int act, int N, long S, int C, int 
     return 0;
 }
 
-constexpr int kTile = 4;               // rows a thread loads at once
-
 static int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 Shape make_shape(int N, long S, int C, int G, int* V, long most_cw) {
@@ -155,6 +153,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_stats(const T* __restrict
         for (int g = tid; g < k.ng; g += kThreads) pivots[(size_t)k.n * sh.G + k.g0 + g] = (double)(float)xn[(size_t)(k.g0 + g) * sh.cg];
     Sums<T, V> sums;
     sums.start(pivot);
+    constexpr int kTile = tile_rows(V, sizeof(T));
     Walk<kTile, false>(sh, k.blk, row, per_pass, on).run(
         [&](long r) {
             Tile<T, V, kTile> t;
@@ -200,6 +199,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
     const auto put = [&](long r, const typename Pack<T, V>::type& vx, const typename Pack<T, V>::type& vr) {
         finish<T, V, ACT, STREAM>(a, vx, vr, has_res, py + (size_t)r * yr.ss, oflag != nullptr, amax);
     };
+    constexpr int kTile = tile_rows(V, sizeof(T));
     const auto rows = [&](auto last) {                     // last rows first: what the sums read last is what the caches hold
         Walk<kTile, true>(sh, k.blk, row, per_pass, row < per_pass).run(
             [&](long r) {
@@ -322,13 +322,13 @@ struct Plan {
 
 static Plan plan_forward(int N, long S, int C, int G, int dtype) {
     Plan p = {};
-    p.V = small_vector_width(C);
+    p.V = vector_width(C);
     p.shape = small_shape(N, S, C, G, &p.V, dtype);
     p.threads = p.shape.nsub > 1 ? 0 : small_threads(p.shape, p.V, &p.M);
     if (!p.threads) {
-        p.V = vector_width(C, dtype);
+        p.V = vector_width(C);
         p.shape = make_shape(N, S, C, G, &p.V, 1l << 40);
-        cut_rows(&p.shape, p.V, kStatsBlocks, kTile, kStatsTiles);
+        cut_rows(&p.shape, p.V, kStatsBlocks, tile_rows(p.V, element_bytes(dtype)), kStatsTiles);
         p.bytes = stats_bytes(p.shape);
     }
     return p;
@@ -341,18 +341,17 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     const T *x = (const T*)f.x, *res = (const T*)f.residual;
     const long grid = (long)sh.N * sh.nblk * sh.chunks;
     const size_t per_table = (sh.cg % V == 0 ? 1 : V) * sizeof(double2);
-    if constexpr (V <= 4)
-        if (p.threads) {
-            const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
-            LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
-            if (p.M == 4)
-                hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
-                                   res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
-            else
-                hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
-                                   res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
-            return check_launch("msnet_group_norm");
-        }
+    if (p.threads) {
+        const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
+        LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
+        if (p.M == 4)
+            hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                               res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+        else
+            hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                               res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+        return check_launch("msnet_group_norm");
+    }
     double2* part = (double2*)ws;
     double* pivots = (double*)(part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G);
     {
@@ -361,7 +360,7 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
         if (int rc = check_launch("msnet_group_norm")) return rc;
     }
     Shape out = sh;
-    cut_rows(&out, V, kApplyBlocks, kTile, kApplyTiles);
+    cut_rows(&out, V, kApplyBlocks, tile_rows(V, sizeof(T)), kApplyTiles);
     const long grid2 = (long)out.N * out.nblk * out.chunks;
     LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
     const auto apply = streams((double)sh.N * m * sh.G * sizeof(T)) ? group_norm_apply<T, V, ACT, true> : group_norm_apply<T, V, ACT, false>;
@@ -378,9 +377,7 @@ static int forward_v(const Forward& f, const Plan& p, int act, void* ws, double 
 
 template <class T>
 static int forward_t(const Forward& f, const Plan& p, int act, void* ws, double bytes) {
-    if constexpr (sizeof(T) == 2)
-        if (p.V == 8) return forward_v<T, 8>(f, p, act, ws, bytes);
-    return p.V == 4 ? forward_v<T, 4>(f, p, act, ws, bytes) : forward_v<T, 1>(f, p, act, ws, bytes);
+    return p.V == 4 ? forward_v<T, 4>(f, p, act, ws, bytes) : p.V == 2 ? forward_v<T, 2>(f, p, act, ws, bytes) : forward_v<T, 1>(f, p, act, ws, bytes);
 }
 
 }  // namespace gn

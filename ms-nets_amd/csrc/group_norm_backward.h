@@ -44,10 +44,8 @@ constexpr int grad_many(int V, int bytes) { return V * bytes == 16 ? 4 : 8; }
 constexpr int kGradTable = 2048;       // sums of the single launch's threads at a time: 32 KB
 constexpr int kParamCols = 16;         // channels of one workgroup that sums dgamma and dbeta
 constexpr long kGradApplyBlocks = 512;
-constexpr long grad_sum_blocks(int V) { return V == 8 ? 512 : 768; }        // two or three of these fit a compute unit's registers
-// rows a thread loads at once (of eight channels the sums' registers leave room for two)
-constexpr int sum_tile(int V) { return V == 8 ? 2 : 4; }
-constexpr int kGradTile = 4;
+constexpr long kGradSumBlocks = 768;   // three of these fit a compute unit's registers
+constexpr int kSumTile = 4;            // rows a thread of the sums loads at once (the sums of eight do not fit beside them)
 constexpr int kGradSumTiles = 2, kGradApplyTiles = 2;  // tiles of a workgroup at least
 
 // What a thread keeps of its V channels.  WHOLE: they lie in one group, whose constants are kept once.
@@ -175,7 +173,6 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
                                                                  const float* __restrict__ bias, const double2* __restrict__ stats, Shape sh,
                                                                  double2* __restrict__ part, double2* __restrict__ chan) {
     extern __shared__ __attribute__((aligned(16))) double2 tab[];      // [kThreads * V] sums, [ng] statistics
-    constexpr int U = sum_tile(V);
     double2* st = tab + kThreads * V;
     const Chunk k = chunk_of(sh, blockIdx.x);
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
@@ -199,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_sums(const T* __rest
         }
     };
     const Inputs<T, V, RES> in(x, xr, dy, yr, residual, rr, k.n, k.c0 + cl);
-    Walk<U, false>(sh, k.blk, row, per_pass, on).run([&](long r) { in.template tile<U, false>(r, per_pass, add); }, [&](long r) { in.row(r, add); });
+    Walk<kSumTile, false>(sh, k.blk, row, per_pass, on).run([&](long r) { in.template tile<kSumTile, false>(r, per_pass, add); }, [&](long r) { in.row(r, add); });
     double2 v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = make_double2(s[e], q[e]);
@@ -247,8 +244,9 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
         if (RES && dresidual) store<T, V, STREAM>(dresidual + dense + (size_t)r * sh.C, dz);
     };
     const Inputs<T, V, RES> in(x, xr, dy, yr, residual, rr, k.n, k.c0 + cl);
-    Walk<kGradTile, true>(sh, k.blk, row, per_pass, row < per_pass).run(             // last rows first, as in the forward
-        [&](long r) { in.template tile<kGradTile, STREAM>(r, per_pass, put); }, [&](long r) { in.row(r, put); });
+    constexpr int kTile = tile_rows(V, sizeof(T));
+    Walk<kTile, true>(sh, k.blk, row, per_pass, row < per_pass).run(             // last rows first, as in the forward
+        [&](long r) { in.template tile<kTile, STREAM>(r, per_pass, put); }, [&](long r) { in.row(r, put); });
 }
 
 // All rows of one chunk of one sample in registers, M vectors of x and of dy a thread.  direct: one sample, its channel sums are
@@ -352,26 +350,25 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     // (a multiple of the eight dies, so that a row's workgroup stays on the die whose cache its sums were read into)
     const unsigned param_blocks = params ? (unsigned)((sh.C + kParamCols - 1) / kParamCols + 7) / 8 * 8 : 0;
     const unsigned grid = (unsigned)((long)sh.N * sh.nblk * sh.chunks);
-    if constexpr (V <= 4)
-        if (p.threads) {
-            const bool direct = sh.N == 1;
-            double2* chan = direct || !params ? nullptr : (double2*)ws;
-            const size_t lds = (kGradTable + sh.cw + 2 * sh.gpc) * sizeof(double2);
-            {
-                LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
-                if (p.M == kGradFew)
-                    hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
-                                       f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
-                else
-                    hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, grad_many(V, sizeof(T)), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
-                                       f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
-                if (int rc = check_launch("msnet_group_norm_backward")) return rc;
-            }
-            if (!chan) return 0;
-            LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.C);
-            hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N, sh.C, f.dweight, f.dbias);
-            return check_launch("msnet_group_norm_backward");
+    if (p.threads) {
+        const bool direct = sh.N == 1;
+        double2* chan = direct || !params ? nullptr : (double2*)ws;
+        const size_t lds = (kGradTable + sh.cw + 2 * sh.gpc) * sizeof(double2);
+        {
+            LaunchScope ls("group_norm_grad_small", f.stream, 16.0 * values, values * sizeof(T) * (RES ? 5 : 3));
+            if (p.M == kGradFew)
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, kGradFew, ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
+            else
+                hipLaunchKernelGGL((group_norm_grad_small<T, V, WHOLE, grad_many(V, sizeof(T)), ACT, RES>), dim3(grid), dim3(p.threads), lds, f.stream, dy, f.yr, x, f.xr, res, f.rr,
+                                   f.weight, f.bias, f.stats, dx, dres, f.dweight, f.dbias, sh, chan, direct, 1. / m);
+            if (int rc = check_launch("msnet_group_norm_backward")) return rc;
         }
+        if (!chan) return 0;
+        LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.C);
+        hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N, sh.C, f.dweight, f.dbias);
+        return check_launch("msnet_group_norm_backward");
+    }
     double2* part = (double2*)ws;
     double2* chan = part + (size_t)sh.N * sh.nblk * sh.nsub * sh.G;
     {
@@ -381,7 +378,7 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
         if (int rc = check_launch("msnet_group_norm_backward")) return rc;
     }
     Shape out = sh;
-    cut_rows(&out, V, kGradApplyBlocks, kGradTile, kGradApplyTiles);
+    cut_rows(&out, V, kGradApplyBlocks, tile_rows(V, sizeof(T)), kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
     LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
     const auto apply = streams(values * sizeof(T)) ? group_norm_grad_apply<T, V, WHOLE, ACT, RES, true> : group_norm_grad_apply<T, V, WHOLE, ACT, RES, false>;
@@ -404,9 +401,7 @@ static int backward_v(const Backward& f, const BackwardPlan& p, int act, void* w
 
 template <class T>
 static int backward_t(const Backward& f, const BackwardPlan& p, int act, void* ws) {
-    if constexpr (sizeof(T) == 2)
-        if (p.V == 8) return backward_v<T, 8>(f, p, act, ws);
-    return p.V == 4 ? backward_v<T, 4>(f, p, act, ws) : backward_w<T, 1, true>(f, p, act, ws);
+    return p.V == 4 ? backward_v<T, 4>(f, p, act, ws) : p.V == 2 ? backward_v<T, 2>(f, p, act, ws) : backward_w<T, 1, true>(f, p, act, ws);
 }
 
 }  // namespace gn

@@ -18,7 +18,7 @@ static int grad_small_threads(const Shape& s, int V, int dtype, int* M) {
 BackwardPlan plan_backward(int N, long S, int C, int G, int dtype) {
     BackwardPlan p = {};
     long w = 64 / element_bytes(dtype);                     // 64-byte row segments, wider ones once workgroups abound (as in the forward)
-    p.V = small_vector_width(C);
+    p.V = vector_width(C);
     p.shape = make_shape(N, S, C, G, &p.V, w);
     while ((long)N * p.shape.chunks > 2048 && w < (long)kThreads * p.V) {
         w *= 2;
@@ -31,9 +31,9 @@ BackwardPlan plan_backward(int N, long S, int C, int G, int dtype) {
     if (p.threads) {
         p.bytes = N > 1 ? (size_t)N * C * sizeof(double2) : 0;
     } else {
-        p.V = vector_width(C, dtype);
+        p.V = vector_width(C);
         p.shape = make_shape(N, S, C, G, &p.V, (long)kThreads * p.V / 2);
-        cut_rows(&p.shape, p.V, grad_sum_blocks(p.V), sum_tile(p.V), kGradSumTiles);
+        cut_rows(&p.shape, p.V, kGradSumBlocks, kSumTile, kGradSumTiles);
         p.bytes = ((size_t)N * p.shape.nblk * p.shape.nsub * G + (size_t)N * p.shape.nblk * C) * sizeof(double2);
     }
     return p;
