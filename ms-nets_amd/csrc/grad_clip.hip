@@ -17,41 +17,67 @@ namespace msnet {
 namespace clip {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 112;          // in a kernel's arguments, which are 4 KB at most
-constexpr int kPart = 140;             // of one launch that writes them to the workspace
+constexpr int kTensors = 176;          // in a kernel's arguments, which are 4 KB at most
+constexpr int kPart = 216;             // of one launch that writes them to the workspace
 constexpr int kChunk = 16384;          // values of a chunk
 constexpr unsigned kBlocks = 1024;     // workgroups at most: four a compute unit, all on the device at once
 
-// One tensor.  n: its length, its input's type in bits 60 and 61, its output's in the top two.
+// One tensor.  n: its length, its input's type in bits 44 and 45, its output's in bits 46 and 47.
 struct Entry { const void* in; void* out; unsigned long n; };
-__host__ __device__ inline unsigned long packed(long n, int in, int out) { return (unsigned long)n | (unsigned long)in << 60 | (unsigned long)out << 62; }
-__device__ __forceinline__ long length(const Entry& e) { return (long)(e.n & ((1ul << 60) - 1)); }
-__device__ __forceinline__ int types(const Entry& e) { return (int)(e.n >> 60); }      // input's + 4 * output's
+constexpr int kLengthBits = 44;
+__device__ __forceinline__ long length(const Entry& e) { return (long)(e.n & ((1ul << kLengthBits) - 1)); }
+__device__ __forceinline__ int types(const Entry& e) { return (int)(e.n >> kLengthBits); }      // input's + 4 * output's
 
-struct Arguments {
-    Entry e[kTensors];
-    unsigned first[kTensors + 1];      // first chunk of each tensor
+// N of them as kernel arguments, 18 bytes each: addresses and n have 48 bits.
+template <int N>
+struct Packed {
+    unsigned in[N], out[N], n[N];
+    unsigned short in_high[N], out_high[N], n_high[N];
+    void set(int i, const void* in_, void* out_, unsigned long n_) {
+        in[i] = (unsigned)(uintptr_t)in_;
+        out[i] = (unsigned)(uintptr_t)out_;
+        n[i] = (unsigned)n_;
+        in_high[i] = (unsigned short)((uintptr_t)in_ >> 32);
+        out_high[i] = (unsigned short)((uintptr_t)out_ >> 32);
+        n_high[i] = (unsigned short)(n_ >> 32);
+    }
+    __device__ __forceinline__ Entry get(int i) const {
+        return {reinterpret_cast<const void*>((uintptr_t)in_high[i] << 32 | in[i]), reinterpret_cast<void*>((uintptr_t)out_high[i] << 32 | out[i]),
+                (unsigned long)n_high[i] << 32 | n[i]};
+    }
+};
+
+// The arguments lie in host memory, across the bus: all of them to LDS at once, 16 bytes a thread, and one wait.
+template <class A>
+__device__ __forceinline__ const A& in_lds(const A& a, uint4* lds, int tid) {
+    static_assert(sizeof(A) % 16 == 0 && sizeof(A) <= 16 * kThreads, "one load a thread");
+    if (tid < (int)(sizeof(A) / 16)) lds[tid] = reinterpret_cast<const uint4*>(&a)[tid];
+    __syncthreads();
+    return *reinterpret_cast<const A*>(lds);
+}
+
+struct alignas(16) Arguments {
+    Packed<kTensors> e;
+    unsigned first[kTensors];          // first chunk of each tensor
     int count;
 };
 
-// Where a workgroup finds its chunks' tensors: the arguments, which lie in host memory, are copied to LDS at once, and a chunk's
-// tensor is the number of first chunks up to it, two a lane.
+// Where a workgroup finds its chunks' tensors: a chunk's is the number of first chunks up to it, three a lane.
 struct ArgumentLookup {
-    Entry* e;
-    unsigned a, b;
-    __device__ __forceinline__ ArgumentLookup(const Arguments& t, Entry* lds) : e(lds) {
-        static_assert(kTensors <= 128, "two a lane");
-        const int tid = threadIdx.x, lane = tid & 63;
-        if (tid < t.count) lds[tid] = t.e[tid];
-        a = lane < t.count ? t.first[lane] : ~0u;
-        b = lane + 64 < t.count ? t.first[lane + 64] : ~0u;
-        __syncthreads();
+    const Arguments& t;
+    unsigned f[3];
+    __device__ __forceinline__ ArgumentLookup(const Arguments& a, uint4* lds) : t(in_lds(a, lds, threadIdx.x)) {
+        static_assert(kTensors <= 192, "three a lane");
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) f[j] = lane + 64 * j < t.count ? t.first[min(lane + 64 * j, kTensors - 1)] : ~0u;
     }
     __device__ __forceinline__ Entry find(unsigned chunk, long* at) const {
-        const int k = __popcll(__ballot(a <= chunk)) + __popcll(__ballot(b <= chunk)) - 1;
-        const unsigned first = k < 64 ? __shfl(a, k) : __shfl(b, k - 64);
-        *at = (long)(chunk - first) * kChunk;
-        return e[k];
+        int k = -1;
+#pragma unroll
+        for (int j = 0; j < 3; ++j) k += __popcll(__ballot(f[j] <= chunk));
+        *at = (long)(chunk - t.first[k]) * kChunk;
+        return t.e.get(k);
     }
 };
 
@@ -63,7 +89,7 @@ struct Workspace {
 
 struct WorkspaceLookup {
     Workspace w;
-    __device__ __forceinline__ WorkspaceLookup(const Workspace& t, Entry*) : w(t) {}
+    __device__ __forceinline__ WorkspaceLookup(const Workspace& t, uint4*) : w(t) {}
     __device__ __forceinline__ Entry find(unsigned chunk, long* at) const {
         const unsigned k = w.tensor[chunk];
         *at = (long)(chunk - w.first[k]) * kChunk;
@@ -75,23 +101,39 @@ template <class Source> struct Lookup;
 template <> struct Lookup<Arguments> { typedef ArgumentLookup type; };
 template <> struct Lookup<Workspace> { typedef WorkspaceLookup type; };
 
-struct Part {
-    Entry e[kPart];
-    unsigned first[kPart + 1];
+struct alignas(16) Part {
+    Packed<kPart> e;
     int count;
 };
-static_assert(sizeof(Arguments) + 64 <= 4096 && sizeof(Part) + 64 <= 4096, "kernel arguments");
+static_assert(sizeof(Arguments) + 64 <= 4096 && sizeof(Part) + 64 <= 4096 && kPart <= kThreads, "kernel arguments, one thread a tensor");
 
-__global__ __launch_bounds__(kThreads) void grad_table(Part p, int at, Entry* __restrict__ e, unsigned* __restrict__ first, unsigned* __restrict__ tensor) {
-    __shared__ unsigned begin[kPart + 1];
+__device__ __forceinline__ unsigned chunks_of(const Entry& e) { return (unsigned)((length(e) + kChunk - 1) / kChunk); }
+
+// Tensors at .. at + count of the list, whose first chunk is `before`, and their chunks' places.
+__global__ __launch_bounds__(kThreads) void grad_table(Part p, int at, unsigned before, Entry* __restrict__ e, unsigned* __restrict__ first,
+                                                       unsigned* __restrict__ tensor) {
+    __shared__ unsigned begin[kThreads + 1], wave[kThreads / 64];
+    __shared__ uint4 lds[sizeof(Part) / 16];
     const int tid = threadIdx.x, lane = tid & 63;
-    if (tid < p.count) { e[at + tid] = p.e[tid]; first[at + tid] = p.first[tid]; }      // (the arguments lie in host memory: one wait for all)
-    if (tid <= p.count) begin[tid] = p.first[tid];
+    Entry mine = {nullptr, nullptr, 0};
+    const Part& q = in_lds(p, lds, tid);
+    if (tid < q.count) mine = q.e.get(tid);
+    const unsigned chunks = tid < q.count ? chunks_of(mine) : 0u;
+    unsigned sum = chunks;                                 // of this tensor's chunks and all before it in the wave
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned v = __shfl_up(sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 63) wave[tid >> 6] = sum;
     __syncthreads();
-    for (int i = tid >> 6; i < p.count; i += kThreads / 64)
+    for (int w = 0; w < tid >> 6; ++w) sum += wave[w];
+    begin[tid + 1] = before + sum;
+    if (tid == 0) begin[0] = before;
+    __syncthreads();
+    if (tid < q.count) { e[at + tid] = mine; first[at + tid] = begin[tid]; }
+    for (int i = tid >> 6; i < q.count; i += kThreads / 64)
         for (unsigned b = begin[i] + lane; b < begin[i + 1]; b += 64) tensor[b] = (unsigned)(at + i);
 }
-static_assert(kPart < kThreads, "one thread a tensor");
 
 template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };      // any view's alignment
 
@@ -121,6 +163,7 @@ __device__ __forceinline__ double square_sum(const T* p, int n, int tid) {
     };
     for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
         const Vec a = v[i], b = v[i + kThreads], c = v[i + 2 * kThreads], d = v[i + 3 * kThreads];
+        __builtin_amdgcn_sched_barrier(0);                 // (all four in flight: the compiler would move each down to its use)
         add(a); add(b); add(c); add(d);
     }
     for (; i < nv; i += kThreads) add(v[i]);
@@ -135,7 +178,7 @@ __device__ __forceinline__ double square_sum(const T* p, int n, int tid) {
 template <class Source>
 __global__ __launch_bounds__(kThreads) void grad_square_sums(Source src, unsigned chunks, double* __restrict__ sums) {
     __shared__ double tab[4];
-    __shared__ Entry lds[kTensors];
+    __shared__ uint4 lds[sizeof(Arguments) / 16];
     const int tid = threadIdx.x;
     const typename Lookup<Source>::type table(src, lds);
     double s = 0.;
@@ -167,34 +210,45 @@ __global__ __launch_bounds__(kThreads) void grad_total(const double* __restrict_
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-template <class T, class O>
+// Vectors of 16 bytes of the output, so that a wave writes whole lines.
+template <bool STREAM, class T, class O>
 __device__ __forceinline__ void scale(const T* p, O* o, int n, float f, int tid) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(O), U = sizeof(T) < sizeof(O) ? 8 : 4;
     typedef typename Pack<T, V>::type Vec;
     typedef typename Pack<O, V>::type Out;
     const int nv = n / V;
     const Vec* v = reinterpret_cast<const Vec*>(p);
     Out* w = reinterpret_cast<Out*>(o);
-    auto put = [&](int i, const Vec& a) {
+    const auto get = [&](int i) {
+        if constexpr (STREAM) return __builtin_nontemporal_load(v + i);
+        else return v[i];
+    };
+    const auto put = [&](int i, const Vec& a) {
         Out r;
 #pragma unroll
         for (int e = 0; e < V; ++e) r[e] = (O)((float)a[e] * f);
-        w[i] = r;
+        if constexpr (STREAM) __builtin_nontemporal_store(r, w + i);
+        else w[i] = r;
     };
     int i = tid;
-    for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
-        const Vec a = v[i], b = v[i + kThreads], c = v[i + 2 * kThreads], d = v[i + 3 * kThreads];
-        put(i, a); put(i + kThreads, b); put(i + 2 * kThreads, c); put(i + 3 * kThreads, d);
+    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
+        Vec a[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[u] = get(i + u * kThreads);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) put(i + u * kThreads, a[u]);
     }
-    for (; i < nv; i += kThreads) put(i, v[i]);
+    for (; i < nv; i += kThreads) put(i, get(i));
     const int at = nv * V + tid;
     if (at < n) o[at] = (O)((float)p[at] * f);
 }
 
-template <class Source>
+// STREAM: past the caches, for gradients that do not fit them anyway.
+template <class Source, bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_scale(Source src, unsigned chunks, const double* __restrict__ sums, double max_norm, float* norm) {
     __shared__ double tab[4];
-    __shared__ Entry lds[kTensors];
+    __shared__ uint4 lds[sizeof(Arguments) / 16];
     const int tid = threadIdx.x;
     const typename Lookup<Source>::type table(src, lds);
     const double total = sqrt(total_of(sums, gridDim.x, tab, tid));
@@ -210,11 +264,11 @@ __global__ __launch_bounds__(kThreads) void grad_scale(Source src, unsigned chun
             const void* p = e.in;
             void* o = e.out;
             switch (types(e)) {
-                case 0: scale(static_cast<const float*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 1: scale(static_cast<const _Float16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 2: scale(static_cast<const __bf16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 5: scale(static_cast<const _Float16*>(p) + at, static_cast<_Float16*>(o) + at, n, f, tid); break;
-                default: scale(static_cast<const __bf16*>(p) + at, static_cast<__bf16*>(o) + at, n, f, tid);
+                case 0: scale<STREAM>(static_cast<const float*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 1: scale<STREAM>(static_cast<const _Float16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 2: scale<STREAM>(static_cast<const __bf16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
+                case 5: scale<STREAM>(static_cast<const _Float16*>(p) + at, static_cast<_Float16*>(o) + at, n, f, tid); break;
+                default: scale<STREAM>(static_cast<const __bf16*>(p) + at, static_cast<__bf16*>(o) + at, n, f, tid);
             }
         }
         if (c < gridDim.x) break;
@@ -230,12 +284,12 @@ struct Cut {
     }
 };
 
-static long chunks_of(int64_t n) { return (long)((n + kChunk - 1) / kChunk); }
+static long chunks_of_length(int64_t n) { return (long)((n + kChunk - 1) / kChunk); }
 
 static Cut cut(const int64_t* n, int count) {
     Cut c = {0, 0};
     for (int i = 0; i < count; ++i) {
-        c.chunks += (unsigned long)chunks_of(n[i]);
+        c.chunks += (unsigned long)chunks_of_length(n[i]);
         c.tensors += n[i] > 0;
     }
     return c;
@@ -272,7 +326,7 @@ using namespace msnet;
 static int check_lengths(const char* what, const int64_t* n, int count) {
     if (count < 0 || (count && !n)) return fail("%s: %d tensors", what, count);
     for (int i = 0; i < count; ++i)
-        if (n[i] < 0 || n[i] > ((int64_t)1 << 48)) return fail("%s: tensor %d has %lld values", what, i, (long long)n[i]);
+        if (n[i] < 0 || n[i] >= ((int64_t)1 << clip::kLengthBits)) return fail("%s: tensor %d has %lld values", what, i, (long long)n[i]);
     return 0;
 }
 
@@ -310,9 +364,10 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
         if (out_host) bytes_out += (double)n_host[i] * (out_types_host[i] ? 2 : 4);
     }
     const unsigned blocks = c.blocks(), chunks = (unsigned)c.chunks;
-    const auto entry = [&](int i) {
-        return clip::Entry{in_host[i], out_host ? out_host[i] : nullptr,
-                           clip::packed(n_host[i], in_types_host[i], out_host ? out_types_host[i] : in_types_host[i])};
+    const bool past_caches = bytes_out >= 64e6;
+    const auto put = [&](auto& packed, int at, int i) {
+        const unsigned long in = in_types_host[i], out = out_host ? out_types_host[i] : in_types_host[i];
+        packed.set(at, in_host[i], out_host ? out_host[i] : nullptr, (unsigned long)n_host[i] | (in + 4 * out) << clip::kLengthBits);
     };
     const auto run = [&](auto src) {
         if (blocks) {
@@ -321,7 +376,8 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
         }
         if (out_host && blocks) {
             LaunchScope ls("grad_scale", s, 0, bytes_in + bytes_out);
-            hipLaunchKernelGGL((clip::grad_scale<decltype(src)>), dim3(blocks), dim3(clip::kThreads), 0, s, src, chunks, sums, max_norm, norm);
+            const auto kernel = past_caches ? clip::grad_scale<decltype(src), true> : clip::grad_scale<decltype(src), false>;
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(clip::kThreads), 0, s, src, chunks, sums, max_norm, norm);
         } else {
             LaunchScope ls("grad_total", s, 0, 8.0 * blocks);
             hipLaunchKernelGGL(clip::grad_total, dim3(1), dim3(clip::kThreads), 0, s, sums, blocks, norm);
@@ -331,12 +387,12 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
     if (c.tensors <= clip::kTensors) {
         clip::Arguments a;
         a.count = 0;
-        a.first[0] = 0;
+        unsigned first = 0;
         for (int i = 0; i < count; ++i)
             if (n_host[i]) {
-                a.e[a.count] = entry(i);
-                a.first[a.count + 1] = a.first[a.count] + (unsigned)clip::chunks_of(n_host[i]);
-                ++a.count;
+                put(a.e, a.count, i);
+                a.first[a.count++] = first;
+                first += (unsigned)clip::chunks_of_length(n_host[i]);
             }
         return run(a);
     }
@@ -347,18 +403,17 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
         LaunchScope ls("grad_table", s, 0, 28.0 * c.tensors + 4.0 * chunks);
         clip::Part p;
         p.count = 0;
-        p.first[0] = 0;
         int at = 0;
+        unsigned before = 0, next = 0;
         for (int i = 0; i < count; ++i) {
             if (n_host[i]) {
-                p.e[p.count] = entry(i);
-                p.first[p.count + 1] = p.first[p.count] + (unsigned)clip::chunks_of(n_host[i]);
-                ++p.count;
+                put(p.e, p.count++, i);
+                next += (unsigned)clip::chunks_of_length(n_host[i]);
             }
             if (p.count == clip::kPart || (i == count - 1 && p.count)) {
-                hipLaunchKernelGGL(clip::grad_table, dim3(1), dim3(clip::kThreads), 0, s, p, at, e, first, tensor);
+                hipLaunchKernelGGL(clip::grad_table, dim3(1), dim3(clip::kThreads), 0, s, p, at, before, e, first, tensor);
                 at += p.count;
-                p.first[0] = p.first[p.count];
+                before = next;
                 p.count = 0;
             }
         }
