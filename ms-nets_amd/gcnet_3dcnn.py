@@ -27,31 +27,43 @@ from .net_init import net_init
 FUSE_INPUT_LAYOUT = os.environ.get("MSNET_FUSE_INPUT_LAYOUT", "0") == "1"
 
 
-def _convbn(cin, cout, stride):
-    return nn.Sequential(nn.Conv3d(cin, cout, 3, stride=stride, padding=1, bias=False), nn.BatchNorm3d(cout))
+def make_norm(norm, groups):
+    """The normalisation layer of a width: "batch" is the reference's; "group" normalises every sample by itself (nn.GroupNorm over
+    `groups` groups of channels, csrc/group_norm.hip), for weights trained one or two pairs at a time."""
+    if norm == "batch":
+        return nn.BatchNorm3d
+    if norm == "group":
+        return lambda c: nn.GroupNorm(groups, c)
+    raise ValueError('norm must be "batch" or "group" (got %r)' % (norm,))
 
 
-def _deconvbn(cin, cout):
+def _convbn(cin, cout, stride, norm=nn.BatchNorm3d):
+    return nn.Sequential(nn.Conv3d(cin, cout, 3, stride=stride, padding=1, bias=False), norm(cout))
+
+
+def _deconvbn(cin, cout, norm=nn.BatchNorm3d):
     return nn.Sequential(nn.ConvTranspose3d(cin, cout, 3, stride=2, padding=1, output_padding=1, bias=False),
-                         nn.BatchNorm3d(cout))
+                         norm(cout))
 
 
 class Conv3DBlock(nn.Module):
     """Parameter container for one encoder level (three conv+BN+ReLU, first with the level's stride);
     gcnet_3dcnn.py:30-44.  The arithmetic is issued by GCNet_CostVolumeAggre.forward."""
 
-    def __init__(self, in_planes, planes, stride=1, kernel_size=3):
+    def __init__(self, in_planes, planes, stride=1, kernel_size=3, norm=nn.BatchNorm3d):
         super().__init__()
         if kernel_size != 3:
             raise ValueError("only kernel_size=3 is built")
-        self.convbn_3d_1 = _convbn(in_planes, planes, stride)
-        self.convbn_3d_2 = _convbn(planes, planes, 1)
-        self.convbn_3d_3 = _convbn(planes, planes, 1)
+        self.convbn_3d_1 = _convbn(in_planes, planes, stride, norm)
+        self.convbn_3d_2 = _convbn(planes, planes, 1, norm)
+        self.convbn_3d_3 = _convbn(planes, planes, 1, norm)
         self.stride = stride
 
 
 class GCNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
-    def __init__(self, maxdisp=192, cbmv_in_planes=8, kernel_size=3, is_quarter_input_size=False):
+    def __init__(self, maxdisp=192, cbmv_in_planes=8, kernel_size=3, is_quarter_input_size=False, norm="batch", norm_groups=8):
+        """norm, norm_groups: "group" puts nn.GroupNorm(norm_groups, C) where the reference has nn.BatchNorm3d (its state_dict has
+        no running statistics then) -- an extension, not part of the parity contract."""
         super().__init__()
         if kernel_size != 3:
             raise ValueError("only kernel_size=3 is built")
@@ -60,16 +72,17 @@ class GCNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
         self.kernel_size = kernel_size
         self.is_quarter_input_size = bool(is_quarter_input_size)
         F = self.F
-        self.conv3dbn_1 = _convbn(cbmv_in_planes, F, 1)
-        self.conv3dbn_2 = _convbn(F, F, 1)
-        self.block_3d_1 = Conv3DBlock(F, 2 * F, stride=2)
-        self.block_3d_2 = Conv3DBlock(2 * F, 2 * F, stride=2)
-        self.block_3d_3 = Conv3DBlock(2 * F, 2 * F, stride=2)
-        self.block_3d_4 = Conv3DBlock(2 * F, 4 * F, stride=2)
-        self.deconvbn1 = _deconvbn(4 * F, 2 * F)
-        self.deconvbn2 = _deconvbn(2 * F, 2 * F)
-        self.deconvbn3 = _deconvbn(2 * F, 2 * F)
-        self.deconvbn4 = _deconvbn(2 * F, F)
+        N = make_norm(norm, norm_groups)
+        self.conv3dbn_1 = _convbn(cbmv_in_planes, F, 1, N)
+        self.conv3dbn_2 = _convbn(F, F, 1, N)
+        self.block_3d_1 = Conv3DBlock(F, 2 * F, stride=2, norm=N)
+        self.block_3d_2 = Conv3DBlock(2 * F, 2 * F, stride=2, norm=N)
+        self.block_3d_3 = Conv3DBlock(2 * F, 2 * F, stride=2, norm=N)
+        self.block_3d_4 = Conv3DBlock(2 * F, 4 * F, stride=2, norm=N)
+        self.deconvbn1 = _deconvbn(4 * F, 2 * F, N)
+        self.deconvbn2 = _deconvbn(2 * F, 2 * F, N)
+        self.deconvbn3 = _deconvbn(2 * F, 2 * F, N)
+        self.deconvbn4 = _deconvbn(2 * F, F, N)
         if self.is_quarter_input_size:   # gcnet_3dcnn.py:88-90
             self.deconv5 = nn.ConvTranspose3d(F, 1, 3, stride=4, padding=1, output_padding=3)
         else:
@@ -150,8 +163,8 @@ class GCNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
 
         def conv(x, name, stride=1, residual=None):
             p = pl[name]
-            return hipops.conv3d_k3(x, p.wpk, p.scale, p.shift, p.co, stride=stride, relu=True, residual=residual,
-                                     f16s=p.f16s, wpk_wd=p.wpk_wd, wpk_wd4=p.wpk_wd4)
+            return p.normed(lambda relu, residual: hipops.conv3d_k3(x, p.wpk, p.scale, p.shift, p.co, stride=stride, relu=relu, residual=residual,
+                                                                    f16s=p.f16s, wpk_wd=p.wpk_wd, wpk_wd4=p.wpk_wd4), True, residual)
 
         def block(x, name, stride):
             x = conv(x, name + ".convbn_3d_1", stride)
@@ -160,13 +173,14 @@ class GCNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
 
         def deconv(x, name, skip):
             p = pl[name]
-            return tap(name, hipops.deconv3d_k3s2(x, p.wpk, p.scale, p.shift, p.co, relu=True, residual=skip, f16s=p.f16s))
+            return tap(name, p.normed(lambda relu, residual: hipops.deconv3d_k3s2(x, p.wpk, p.scale, p.shift, p.co, relu=relu, residual=residual,
+                                                                                  f16s=p.f16s), True, skip))
 
         with torch.no_grad():
             p1 = pl["conv3dbn_1"]
             if channels_last:
                 if p1.f16s and cv.shape[4] == 8 and p1.co in (32, 64):
-                    x = hipops.conv3d_c8_in(cv, p1.wpk, p1.scale, p1.shift, p1.co, relu=True)     # range check of the input inside
+                    x = p1.normed(lambda relu, _: hipops.conv3d_c8_in(cv, p1.wpk, p1.scale, p1.shift, p1.co, relu=relu), True)     # range check of the input inside
                 elif not p1.f16s:
                     # fp32 precision: the volume already is the fp32 kernels' input layout and there is no fp16 range to guard
                     # (this branch used to permute + convert -- two passes over the volume -- for nothing)
@@ -176,7 +190,7 @@ class GCNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
                     x = conv(hipops.check_input_range(cv), "conv3dbn_1")
             elif p1.f16s and cv.shape[1] == 8 and p1.co in (32, 64) and FUSE_INPUT_LAYOUT:
                 # the first layer reads the NCDHW volume itself: no layout-conversion pass over the 401 MB
-                x = tap("conv3dbn_1", hipops.conv3d_c8_ncdhw(cv, p1.wpk, p1.scale, p1.shift, p1.co, relu=True))
+                x = tap("conv3dbn_1", p1.normed(lambda relu, _: hipops.conv3d_c8_ncdhw(cv, p1.wpk, p1.scale, p1.shift, p1.co, relu=relu), True))
             else:
                 x = hipops.ncdhw_to_ndhwc(cv)
                 x = tap("conv3dbn_1", conv(x, "conv3dbn_1"))

@@ -901,7 +901,8 @@ def _with_arena(module, run, prec):
 
 class ConvBNPlan:
     """Device-side constants of one conv(+BN) layer: MFMA-packed weight and the eval-mode BN affine
-    y = x*scale + shift with scale = gamma/sqrt(var+eps), shift = beta - mean*scale."""
+    y = x*scale + shift with scale = gamma/sqrt(var+eps), shift = beta - mean*scale.  With a GroupNorm in BN's place the conv runs
+    bare and group_norm, in place behind it, takes over its epilogue's ReLU and residual."""
 
     def __init__(self, conv, bn=None, transposed=False, precision=None):
         w = conv.weight.detach()
@@ -910,6 +911,12 @@ class ConvBNPlan:
         stride = conv.stride[0]
         precision = precision or _default_precision
         lib = _lib.load()
+        self.group_norm = None
+        if isinstance(bn, torch.nn.GroupNorm):
+            # statistics of the sample itself: nothing to fold, the layer runs behind the conv (normed)
+            f32 = lambda p: None if p is None else p.detach().float().contiguous()      # noqa: E731
+            self.group_norm = (bn.num_groups, f32(bn.weight), f32(bn.bias), bn.eps)
+            bn = None
         if precision != "split-fp16":
             self.f16s = False
         elif transposed:
@@ -957,6 +964,15 @@ class ConvBNPlan:
             wf_ = w.float()
             self.wpk_wd4 = [[winograd_depth_weights(wf_[32 * hh:32 * hh + 32, 32 * cc:32 * cc + 32].contiguous()) for cc in range(2)]
                             for hh in range(2)]
+
+
+    def normed(self, conv, relu, residual=None):
+        """conv(relu, residual), the layer's kernel, or conv(False, None) and the group norm."""
+        if self.group_norm is None:
+            return conv(relu, residual)
+        y = conv(False, None)
+        groups, weight, bias, eps = self.group_norm
+        return group_norm(y, groups, weight, bias, eps=eps, act="relu" if relu else "none", residual=residual, out=y)
 
 
 def _registered_tensors(module):

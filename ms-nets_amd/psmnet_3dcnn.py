@@ -16,53 +16,56 @@ import torch
 import torch.nn as nn
 
 from . import hipops
+from .gcnet_3dcnn import make_norm
 from .net_init import net_init
 
 
-def _convbn(cin, cout, stride):
-    return nn.Sequential(nn.Conv3d(cin, cout, 3, stride=stride, padding=1, bias=False), nn.BatchNorm3d(cout))
+def _convbn(cin, cout, stride, norm=nn.BatchNorm3d):
+    return nn.Sequential(nn.Conv3d(cin, cout, 3, stride=stride, padding=1, bias=False), norm(cout))
 
 
-def _deconvbn(cin, cout):
+def _deconvbn(cin, cout, norm=nn.BatchNorm3d):
     return nn.Sequential(nn.ConvTranspose3d(cin, cout, 3, padding=1, output_padding=1, stride=2, bias=False),
-                         nn.BatchNorm3d(cout))
+                         norm(cout))
 
 
 class hourglass(nn.Module):
     """Parameter container of one hourglass (psmnet_3dcnn.py:47-67); arithmetic in PSMNet_CostVolumeAggre."""
 
-    def __init__(self, inplanes):
+    def __init__(self, inplanes, norm=nn.BatchNorm3d):
         super().__init__()
         c = inplanes
-        self.conv1 = nn.Sequential(_convbn(c, 2 * c, 2), nn.ReLU(inplace=True))
-        self.conv2 = _convbn(2 * c, 2 * c, 1)
-        self.conv3 = nn.Sequential(_convbn(2 * c, 2 * c, 2), nn.ReLU(inplace=True))
-        self.conv4 = nn.Sequential(_convbn(2 * c, 2 * c, 1), nn.ReLU(inplace=True))
-        self.conv5 = _deconvbn(2 * c, 2 * c)
-        self.conv6 = _deconvbn(2 * c, c)
+        self.conv1 = nn.Sequential(_convbn(c, 2 * c, 2, norm), nn.ReLU(inplace=True))
+        self.conv2 = _convbn(2 * c, 2 * c, 1, norm)
+        self.conv3 = nn.Sequential(_convbn(2 * c, 2 * c, 2, norm), nn.ReLU(inplace=True))
+        self.conv4 = nn.Sequential(_convbn(2 * c, 2 * c, 1, norm), nn.ReLU(inplace=True))
+        self.conv5 = _deconvbn(2 * c, 2 * c, norm)
+        self.conv6 = _deconvbn(2 * c, c, norm)
 
 
-def _classif():
-    return nn.Sequential(_convbn(32, 32, 1), nn.ReLU(inplace=True),
+def _classif(norm):
+    return nn.Sequential(_convbn(32, 32, 1, norm), nn.ReLU(inplace=True),
                          nn.Conv3d(32, 1, kernel_size=3, padding=1, stride=1, bias=False))
 
 
 class PSMNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
-    def __init__(self, maxdisp, in_planes=64):
+    def __init__(self, maxdisp, in_planes=64, norm="batch", norm_groups=8):
         """in_planes: channels of the input volume.  64 is the reference (a PSMNet feature-concat volume,
         psmnet_3dcnn.py:97); 8 (or 16) lets the aggregator take the matching-space volume directly, which the reference's
-        class cannot (SURVEY defect D3) -- an extension, not part of the parity contract."""
+        class cannot (SURVEY defect D3) -- an extension, not part of the parity contract.
+        norm, norm_groups: as in GCNet_CostVolumeAggre, another one."""
         super().__init__()
+        N = make_norm(norm, norm_groups)
         self.maxdisp = maxdisp
         self.in_planes = int(in_planes)
-        self.dres0 = nn.Sequential(_convbn(self.in_planes, 32, 1), nn.ReLU(inplace=True), _convbn(32, 32, 1), nn.ReLU(inplace=True))
-        self.dres1 = nn.Sequential(_convbn(32, 32, 1), nn.ReLU(inplace=True), _convbn(32, 32, 1))
-        self.dres2 = hourglass(32)
-        self.dres3 = hourglass(32)
-        self.dres4 = hourglass(32)
-        self.classif1 = _classif()
-        self.classif2 = _classif()
-        self.classif3 = _classif()
+        self.dres0 = nn.Sequential(_convbn(self.in_planes, 32, 1, N), nn.ReLU(inplace=True), _convbn(32, 32, 1, N), nn.ReLU(inplace=True))
+        self.dres1 = nn.Sequential(_convbn(32, 32, 1, N), nn.ReLU(inplace=True), _convbn(32, 32, 1, N))
+        self.dres2 = hourglass(32, N)
+        self.dres3 = hourglass(32, N)
+        self.dres4 = hourglass(32, N)
+        self.classif1 = _classif(N)
+        self.classif2 = _classif(N)
+        self.classif3 = _classif(N)
         net_init(self)
         # per-device state (packed-weight plans, activation arena, range guard, captured graphs): hipops.ModuleState
         self._init_device_state()
@@ -109,12 +112,13 @@ class PSMNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
 
         def conv(x, name, stride=1, relu=True, residual=None):
             p = pl[name]
-            return hipops.conv3d_k3(x, p.wpk, p.scale, p.shift, p.co, stride=stride, relu=relu, residual=residual,
-                                     f16s=p.f16s, wpk_wd=p.wpk_wd, wpk_wd4=p.wpk_wd4)
+            return p.normed(lambda relu, residual: hipops.conv3d_k3(x, p.wpk, p.scale, p.shift, p.co, stride=stride, relu=relu, residual=residual,
+                                                                    f16s=p.f16s, wpk_wd=p.wpk_wd, wpk_wd4=p.wpk_wd4), relu, residual)
 
         def deconv(x, name, relu, residual):
             p = pl[name]
-            return hipops.deconv3d_k3s2(x, p.wpk, p.scale, p.shift, p.co, relu=relu, residual=residual, f16s=p.f16s)
+            return p.normed(lambda relu, residual: hipops.deconv3d_k3s2(x, p.wpk, p.scale, p.shift, p.co, relu=relu, residual=residual, f16s=p.f16s),
+                            relu, residual)
 
         def hour(x, name, presqu, postsqu, skip):
             # psmnet_3dcnn.py:69-89; `skip` (= cost0) is the "+ cost0" the caller adds to the hourglass output
@@ -130,13 +134,13 @@ class PSMNet_CostVolumeAggre(hipops.DeviceStateMixin, nn.Module):
         from .gcnet_3dcnn import FUSE_INPUT_LAYOUT
         if channels_last:                    # forward_ndhwc: the 8-plane MS volume as VolumeBuilder(layout="ndhwc") writes it
             if p0.f16s and cost.shape[4] == 8 and p0.co in (32, 64):
-                c0 = conv(hipops.conv3d_c8_in(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=True), "dres0.2")
+                c0 = conv(p0.normed(lambda relu, _: hipops.conv3d_c8_in(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=relu), True), "dres0.2")
             elif not p0.f16s:                # fp32 precision: already the kernels' layout, no fp16 range to guard
                 c0 = conv(conv(cost.contiguous(), "dres0.0"), "dres0.2")
             else:                            # other widths on split-fp16 (the reference's 64 planes): the range check rides in dres0.0's loaders
-                c0 = conv(hipops.conv3d_k3_in(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=True), "dres0.2")
+                c0 = conv(p0.normed(lambda relu, _: hipops.conv3d_k3_in(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=relu), True), "dres0.2")
         elif FUSE_INPUT_LAYOUT and p0.f16s and cost.shape[1] == 8 and p0.co in (32, 64):      # the MS volume: first layer straight from NCDHW
-            c0 = conv(hipops.conv3d_c8_ncdhw(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=True), "dres0.2")
+            c0 = conv(p0.normed(lambda relu, _: hipops.conv3d_c8_ncdhw(cost, p0.wpk, p0.scale, p0.shift, p0.co, relu=relu), True), "dres0.2")
         else:
             c0 = conv(conv(hipops.ncdhw_to_ndhwc(cost), "dres0.0"), "dres0.2")
         cost0 = tap("cost0", conv(conv(c0, "dres1.0"), "dres1.2", relu=False, residual=c0))

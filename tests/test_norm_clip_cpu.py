@@ -6,6 +6,8 @@ import torch
 
 import msnets_amd  # noqa: F401
 from msnets_amd import driver_utils, hipops
+from msnets_amd.gcnet_3dcnn import GCNet_CostVolumeAggre
+from msnets_amd.psmnet_3dcnn import PSMNet_CostVolumeAggre
 
 FAKE = ctypes.c_void_p(1 << 20)              # never read: every call below fails on the host
 
@@ -92,3 +94,19 @@ def test_dense_in_any_order():
     t = torch.zeros(4, 6, 2, 3, 5)
     assert hipops._is_dense(t) and hipops._is_dense(t.to(memory_format=torch.channels_last_3d)) and hipops._is_dense(t.transpose(0, 3))
     assert not hipops._is_dense(t[:, ::2]) and not hipops._is_dense(t[:1].expand(4, 6, 2, 3, 5)) and hipops._is_dense(t[:, :1, :1, :1, :1].contiguous())
+
+
+def test_group_normalised_aggregators():
+    """norm="group": no running statistics, the same keys otherwise, the same convs from the same seed; a bad norm is refused."""
+    for make in (lambda **k: GCNet_CostVolumeAggre(32, **k), lambda **k: PSMNet_CostVolumeAggre(32, **k)):
+        batch, group = make().state_dict(), make(norm="group").state_dict()
+        assert {k for k in batch if "running" not in k and "num_batches" not in k} == set(group)
+        with pytest.raises(ValueError, match="norm must be"):
+            make(norm="layer")
+        with pytest.raises(ValueError):
+            make(norm="group", norm_groups=7)
+    torch.manual_seed(0)
+    a = GCNet_CostVolumeAggre(32).state_dict()
+    torch.manual_seed(0)
+    b = GCNet_CostVolumeAggre(32, norm="group").state_dict()
+    assert all(torch.equal(a[k], b[k]) for k in b), "the same seed gives the same convs"
