@@ -15,9 +15,6 @@ LIB = os.path.join(HERE, "libmsnet_hip.so")
 HOST = os.path.join(HERE, "_host.so")                 # Python module: torch operators over the C ABI (csrc/host_ops.cpp)
 ARCH = "gfx950"
 
-# gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself.
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
 # (source, extra flags).  volume.hip reproduces float32 operation order => no FMA contraction there.
 SOURCES = [
     ("api.cpp", []),
@@ -35,17 +32,19 @@ SOURCES = [
     ("conv3d_f16s_wd.hip", []),
     ("tail.hip", []),
     ("metrics.hip", []),
-    ("group_norm.hip", NO_PACKED_FP32),
-    ("group_norm_backward.hip", NO_PACKED_FP32),
-    ("group_norm_backward_f16.hip", NO_PACKED_FP32),
-    ("group_norm_backward_bf16.hip", NO_PACKED_FP32),
-    ("grad_clip.hip", NO_PACKED_FP32),
+    ("group_norm.hip", []),
+    ("group_norm_backward.hip", []),
+    ("group_norm_backward_f16.hip", []),
+    ("group_norm_backward_bf16.hip", []),
+    ("grad_clip.hip", []),
     ("volume.hip", ["-ffp-contract=off"]),
     # -fno-slp-vectorize: hipcc otherwise packs the ZSAD add chains into v_pk_add_f32 + v_and (no |x| modifier) + v_mov
     ("volume_fused.hip", ["-ffp-contract=off", "-fno-slp-vectorize"]),
 ]
 COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-Wall", "-Wno-unused-function",
-          "-fno-gpu-rdc"]
+          "-fno-gpu-rdc",
+          # gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
