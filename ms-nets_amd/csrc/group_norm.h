@@ -185,6 +185,16 @@ __device__ __forceinline__ void sum_slots(const double2* __restrict__ part, int 
     }
 }
 
+// V channels' gamma or beta, the default's where there are none.  One load from an address chosen before: a load in a branch is waited
+// for at the branch's end, and with it everything else in flight.
+static __device__ const float kDefaults[8] = {0.f, 0.f, 0.f, 0.f, 1.f, 1.f, 1.f, 1.f};
+template <int V>
+__device__ __forceinline__ void load_params(const float* params, int c, bool one, float (&out)[V]) {
+    const auto v = load_raw<float, V>(params ? params + c : kDefaults + (one ? 4 : 0));
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = element<float, V>(v, e);
+}
+
 __device__ __forceinline__ float silu_gate(float z) {       // 1 / (1 + e^-z)
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * z));
 }

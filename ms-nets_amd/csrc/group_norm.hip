@@ -67,11 +67,8 @@ struct Affine {
     float mean[V], scale[V], shift[V];
     // gamma and beta first, so that they arrive while the sums are formed
     __device__ __forceinline__ void load(int c, const float* weight, const float* bias) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            scale[e] = weight ? weight[c + e] : 1.f;
-            shift[e] = bias ? bias[c + e] : 0.f;
-        }
+        load_params<V>(weight, c, true, scale);
+        load_params<V>(bias, c, false, shift);
     }
     __device__ __forceinline__ void set(const double2* st, int c_local, int cg, bool whole) {
         double2 t = st[c_local / cg];
@@ -188,9 +185,11 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
     T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
     Affine<V> a;
     a.load(k.c0 + cl, weight, bias);
+    const double* mine = pivots + (size_t)k.n * sh.G + k.g0;
+    const double pivot = mine[min(tid, k.ng - 1)];         // of the group whose sums this thread will have (of the first kThreads groups)
     sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid, [&](int g, double2 sum) {
         const size_t at = (size_t)k.n * sh.G + k.g0 + g;
-        const double2 v = statistics(sum, pivots[at], inv, eps);
+        const double2 v = statistics(sum, g < kThreads ? pivot : mine[g], inv, eps);
         st[g] = v;
         if (stats && k.blk == 0 && k.sub == 0) stats[at] = v;
     });
@@ -230,7 +229,7 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
     const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
     const int row = tid / cv, cl = (tid % cv) * V;
     const bool whole = sh.cg % V == 0, on = row < per_pass;
-    double2* st = tab + (whole ? threads : threads * V);
+    double2* st = tab + (whole ? threads : threads * V);  // [ng]: first each group's pivot, then its statistics
     const T* xn = x + (size_t)k.n * xr.sn;
     const T* px = xn + k.c0 + cl;
     const int S = (int)sh.S;
@@ -244,6 +243,8 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
         if (on && row + i * per_pass < S) v[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
     Affine<V> a;
     a.load(k.c0 + cl, weight, bias);
+    loads_issued();
+    for (int g = tid; g < k.ng; g += threads) st[g].x = (double)(float)xn[(size_t)(k.g0 + g) * sh.cg];
     Sums<T, V> sums;
     sums.start(pivot);
 #pragma unroll
@@ -251,23 +252,30 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
         if (on && row + i * per_pass < S) sums.add(v[i]);
     sums.join(tab, whole, cv, on, tid, threads);
     sum_groups(tab, (whole ? cv : k.cw) / k.ng, k.ng, tid, threads, [](int, double2 u) { return u; }, [&](int g, double2 sum) {
-        const double2 t = statistics(sum, (double)(float)xn[(size_t)(k.g0 + g) * sh.cg], inv, eps);
+        const double2 t = statistics(sum, st[g].x, inv, eps);
         st[g] = t;
         if (stats) stats[(size_t)k.n * sh.G + k.g0 + g] = t;
     });
     __syncthreads();                                       // statistics are there, and nobody reads x any more (y may be x)
     if (!on) return;
     a.set(st, cl, sh.cg, whole);
-    const T* pr = residual ? residual + (size_t)k.n * rr.sn + k.c0 + cl : nullptr;
+    const bool has_res = residual != nullptr;
+    const T* pr = has_res ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
     T* py = y + (size_t)k.n * yr.sn + k.c0 + cl;
     unsigned amax = 0u;
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
-        const int r = row + i * per_pass;
-        if (r < S) {
-            auto w = v[i];
-            if (residual) w = load_raw<T, V>(pr + (size_t)r * rr.ss);
-            finish<T, V, ACT, false>(a, v[i], w, residual != nullptr, py + (size_t)r * yr.ss, oflag != nullptr, amax);
+    for (int i0 = 0; i0 < M; i0 += 4) {
+        typename Pack<T, V>::type w[4];
+        if (has_res) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (row + (i0 + j) * per_pass < S) w[j] = load_raw<T, V>(pr + (size_t)(row + (i0 + j) * per_pass) * rr.ss);
+            loads_issued();
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = row + (i0 + j) * per_pass;
+            if (r < S) finish<T, V, ACT, false>(a, v[i0 + j], has_res ? w[j] : v[i0 + j], has_res, py + (size_t)r * yr.ss, oflag != nullptr, amax);
         }
     }
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);

@@ -54,11 +54,8 @@ struct Channels {
     static constexpr int W = WHOLE ? 1 : V;
     float mean[W], rstd[W], lo[W], gamma[V], beta[V];
     __device__ __forceinline__ void load(int c, const float* weight, const float* bias) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            gamma[e] = weight ? weight[c + e] : 1.f;
-            beta[e] = bias ? bias[c + e] : 0.f;
-        }
+        load_params<V>(weight, c, true, gamma);
+        load_params<V>(bias, c, false, beta);
     }
     __device__ __forceinline__ void set(const double2* st, int c_local, int cg) {
 #pragma unroll
@@ -226,11 +223,14 @@ __global__ __launch_bounds__(kThreads) void group_norm_grad_apply(const T* __res
     double2 *st = tab + kThreads, *coef = st + k.ng;
     const int tid = threadIdx.x, cv = k.cw / V, per_pass = kThreads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = k.ng > 1 ? sh.cg : k.cw;
-    for (int g = tid; g < k.ng; g += kThreads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
     Channels<V, WHOLE> a;
     a.load(k.c0 + cl, weight, bias);
-    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid,
-              [&](int g, double2 sum) { coef[g] = make_double2(sum.x * inv, sum.y * inv); });
+    const double2* mine = stats + (size_t)k.n * sh.G + k.g0;
+    const double2 first = mine[min(tid, k.ng - 1)];        // of the group whose sums this thread will have (of the first kThreads groups)
+    sum_slots(part + (size_t)k.n * slots * sh.G, slots, sh.G, k.g0, k.ng, tab, tid, [&](int g, double2 sum) {
+        coef[g] = make_double2(sum.x * inv, sum.y * inv);
+        st[g] = g < kThreads ? first : mine[g];
+    });
     a.set(st, cl, cg);
     float c1[WHOLE ? 1 : V], c2[WHOLE ? 1 : V];
 #pragma unroll
@@ -263,7 +263,6 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
     const int tid = threadIdx.x, threads = blockDim.x, cv = k.cw / V, per_pass = threads / cv;
     const int row = tid / cv, cl = (tid % cv) * V, cg = sh.cg;
     const int S = (int)sh.S;
-    for (int g = tid; g < k.ng; g += threads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
     const T* px = x + (size_t)k.n * xr.sn + k.c0 + cl;
     const T* pd = dy + (size_t)k.n * yr.sn + k.c0 + cl;
     const T* pr = RES ? residual + (size_t)k.n * rr.sn + k.c0 + cl : px;
@@ -276,11 +275,12 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
                 vx[i] = load_raw<T, V>(px + (size_t)(row + i * per_pass) * xr.ss);
                 vd[i] = load_raw<T, V>(pd + (size_t)(row + i * per_pass) * yr.ss);
                 if constexpr (RES) vr[i] = load_raw<T, V>(pr + (size_t)(row + i * per_pass) * rr.ss);
-                else vr[i] = vx[i];
             }
     }
     Channels<V, WHOLE> a;
     a.load(k.c0 + cl, weight, bias);
+    loads_issued();
+    for (int g = tid; g < k.ng; g += threads) st[g] = stats[(size_t)k.n * sh.G + k.g0 + g];
     __syncthreads();
     a.set(st, cl, cg);
     double2 v[V];
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
     for (int i = 0; i < M; ++i)
         if (on && row + i * per_pass < S) {
             float dz[V], xhat[V];
-            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], RES ? vr[i] : vx[i], dz, xhat);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[e].x += (double)dz[e];
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(1024) void group_norm_grad_small(const T* __restric
         const int r = row + i * per_pass;
         if (r < S) {
             float dz[V], xhat[V], o[V];
-            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], vr[i], dz, xhat);
+            derive<T, V, WHOLE, ACT, RES>(a, st, cl, cg, vx[i], vd[i], RES ? vr[i] : vx[i], dz, xhat);
             grad_input<V, WHOLE>(a, c1, c2, dz, xhat, o);
             if (dx) store<T, V>(dx + dense + (size_t)r * sh.C, o);
             if (RES && dresidual) store<T, V>(dresidual + dense + (size_t)r * sh.C, dz);
