@@ -377,6 +377,11 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
                            f.yr, x, f.xr, res, f.rr, f.weight, f.bias, f.stats, sh, part, chan);
         if (int rc = check_launch("msnet_group_norm_backward")) return rc;
     }
+    if (!dx && !dres) {                                    // the parameters' gradients alone
+        LaunchScope ls("group_norm_param_grads", f.stream, 0, 16.0 * sh.N * sh.nblk * sh.C);
+        hipLaunchKernelGGL(group_norm_param_grads<0>, dim3(param_blocks), dim3(kThreads), 0, f.stream, chan, (long)sh.N * sh.nblk, sh.C, f.dweight, f.dbias);
+        return check_launch("msnet_group_norm_backward");
+    }
     Shape out = sh;
     cut_rows(&out, V, kGradApplyBlocks, tile_rows(V, sizeof(T)), kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;

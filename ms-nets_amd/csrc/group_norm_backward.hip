@@ -55,6 +55,7 @@ extern "C" int msnet_group_norm_backward(const void* dy, const void* x, const fl
                                          size_t workspace_bytes, msnet_stream_t stream) {
     if (int rc = gn::check_shape("msnet_group_norm_backward", dtype, act, N, S, C, G, 0.)) return rc;
     hipStream_t s = (hipStream_t)stream;
+    if (!dx && !dresidual && !dweight && !dbias) return 0;
     if (N == 0 || S == 0) {                                // no rows: the parameters' gradients are zero
         if (!dweight && !dbias) return 0;
         LaunchScope ls("group_norm_param_grads", s, 0, 8.0 * C);

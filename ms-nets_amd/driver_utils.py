@@ -112,7 +112,8 @@ def clip_grad_norm_(parameters, max_norm):
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)                            # as torch's: nothing says which device
-    return hipops.clip_grads(grads, max_norm)
+    with torch.no_grad():                                   # (gradients that carry a graph of their own are scaled all the same)
+        return hipops.clip_grads(grads, max_norm)
 
 
 def strip_module_prefix(state_dict):

@@ -511,6 +511,8 @@ def _check_norm_args(x, groups, weight, bias, eps, act, residual):
     if x.dim() < 2:
         raise ValueError("x must be channels-last [N, ..., C] (got %s)" % (tuple(x.shape),))
     c = x.shape[-1]
+    if max(x.shape[0], c) >= 1 << 31:
+        raise ValueError("x has %d samples of %d channels: fewer than 2^31 of either are taken" % (x.shape[0], c))
     if isinstance(groups, bool) or int(groups) != groups or groups < 1 or c < 1 or c % int(groups):
         raise ValueError("groups=%r does not divide the %d channels" % (groups, c))
     if act not in _ACT_CODES:
@@ -554,10 +556,12 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
         y = _lib.load_host().group_norm(x, groups, weight, bias, eps, _ACT_CODES[act], residual)
         assert y is not None
         return y
+    given = None
     n, s, c = x.shape[0], (x.numel() // (x.shape[0] * x.shape[-1]) if x.numel() else 0), x.shape[-1]
     if out is None:
         out = _new(x.shape, x.device)
     else:
+        given = out
         _require_gpu(out, "out")
         strides = _row_strides(out)
         if out.shape != x.shape or out.dtype != x.dtype or strides is None or (s > 1 and strides[1] < c) or (n > 1 and strides[0] < (s - 1) * strides[1] + c):
@@ -569,6 +573,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
     lib, code, xs, ys, rs = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(out), _row_strides(residual) if residual is not None else (0, 0)
     nbytes = lib.msnet_group_norm_workspace_bytes(code, n, s, c, groups)
     ws = None if not nbytes else _new(((nbytes + 3) // 4,), x.device) if _tls.arena is not None else torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    if given is not None:
+        torch.autograd.graph.increment_version(given)       # written behind autograd's back: what saved it finds out
     check(lib.msnet_group_norm(ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(out), None, code, _ACT_CODES[act], n, s, c, groups, eps, *xs, *rs, *ys,
                                ptr(ws), nbytes, stream_ptr()), "msnet_group_norm")
     return out

@@ -145,6 +145,18 @@ def test_parameters(gpu):
     check([torch.full((3,), 2.0, device="cuda")], [one.grad], 1.0, driver_utils.clip_grad_norm_(one, 1.0))
 
 
+def test_gradients_with_a_graph(gpu):
+    """Of a loss whose gradient is to be differentiated: clipped by the driver's function, refused where a graph would record it."""
+    p = torch.nn.Parameter(torch.tensor([3.0, 4.0], device="cuda"))
+    p.square().sum().backward(create_graph=True)
+    assert p.grad.requires_grad
+    with pytest.raises(ValueError, match="requires a gradient"):
+        hipops.clip_grads([p.grad], 1.0)
+    old = p.grad.detach().clone()
+    check([old], [p.grad.detach()], 1.0, driver_utils.clip_grad_norm_([p], 1.0))
+    p.grad = None
+
+
 def test_captured_and_replayed(gpu):
     lengths = [100_000, 7, 64] + [33] * 200                     # more tensors than one launch takes
     ts = tensors(lengths, [F32, BF16])

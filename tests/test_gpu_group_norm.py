@@ -258,6 +258,29 @@ def test_partial_gradients(gpu):
         assert torch.equal(one, full[i]), NAMES[i]
 
 
+def test_parameters_alone(gpu):
+    """Frozen inputs: the same dgamma and dbeta, with one sample and with several, in one launch's reach and beyond it."""
+    for shape in ((1, 40, 16), (3, 40, 16), (1, 30000, 16), (2, 30000, 16)):
+        x, w, b, r, dy = make(shape, F32, True)
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        full = torch.autograd.grad(hipops.group_norm(leaves[0], 4, *leaves[1:3], act="relu", residual=leaves[3]), leaves, dy)
+        both = torch.autograd.grad(hipops.group_norm(x, 4, *leaves[1:3], act="relu", residual=r), leaves[1:3], dy)
+        assert torch.equal(both[0], full[1]) and torch.equal(both[1], full[2])
+    dr, = torch.autograd.grad(hipops.group_norm(x, 4, w, b, residual=leaves[3]), [leaves[3]], dy)
+    assert torch.equal(dr, dy)                 # without an activation
+
+
+def test_out_is_seen_by_autograd(gpu):
+    x, w, b, _, _ = make((1, 20, 8), F32, False)
+    leaf = x.clone().requires_grad_()
+    mid = leaf * 1
+    loss = mid.square().sum()                  # keeps mid
+    with torch.no_grad():
+        hipops.group_norm(mid, 2, w, b, out=mid)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals_on_the_gpu(gpu):
     x, w, b, r, _ = make((2, 10, 12), F32, True)
     call = hipops.group_norm
