@@ -7,11 +7,13 @@
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <vector>
 
@@ -91,6 +93,18 @@ Tensor forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const 
                          (int)groups, eps, xr.sample, xr.row, rr.sample, rr.row, d.s * d.c, d.c, data(ws), bytes, stream_of(x.get_device())),
             "msnet_group_norm");
     return y;
+}
+
+// While a stream is captured, a leaf must not still be held by a graph that was recorded on another stream: its accumulation node
+// belongs to that stream, the captured backward would make the two wait for each other, and torch ends the process there.
+void check_capture(const Tensor& t) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const auto theirs = node->stream();
+    TORCH_CHECK(!theirs || *theirs == c10::hip::getCurrentHIPStream(t.get_device()).unwrap(),
+                "group_norm is being captured while a graph recorded on another stream still holds one of its leaves: drop the results of earlier "
+                "eager steps on these tensors first");
 }
 
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
@@ -178,6 +192,8 @@ PyObject* group_norm(PyObject*, PyObject* args) {
     if (r.defined() && (!ordinary(r, device) || r.scalar_type() != x.scalar_type() || r.sizes() != x.sizes() || !rows_of(r, &any))) Py_RETURN_NONE;
     const bool grad = c10::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()) ||
                                                       (r.defined() && r.requires_grad()));
+    if (grad && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+        for (const Tensor* t : {&x, &w, &b, &r}) check_capture(*t);
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     return THPVariable_Wrap(grad ? GroupNorm::apply(x, given(w), given(b), given(r), (int64_t)groups, eps, (int64_t)act)
                                  : forward(x, w, b, r, groups, eps, act, Tensor()));

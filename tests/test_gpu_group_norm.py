@@ -233,6 +233,25 @@ def test_captured_and_replayed(gpu, shape):
         assert all(torch.equal(a, c) for a, c in zip(got, step())), seed
 
 
+def test_capture_beside_a_live_eager_graph_is_refused(gpu):
+    """Captured while an eager graph of the same leaves lives, a backward pass would end the process: the forward refuses."""
+    x, w, b, _, dy = make((1, 60, 16), F32, False)
+    leaf = x.clone().requires_grad_()
+    alive = hipops.group_norm(leaf, 4, w, b, act="relu")
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="drop the results"):
+        with torch.cuda.graph(graph):
+            hipops.group_norm(leaf, 4, w, b, act="relu")
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, = torch.autograd.grad(hipops.group_norm(leaf, 4, w, b, act="relu"), leaf, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = dx.clone()
+    assert torch.equal(got, torch.autograd.grad(hipops.group_norm(leaf, 4, w, b, act="relu"), leaf, dy)[0])
+
+
 def test_saved_tensors_are_watched_and_differentiated_once(gpu):
     x, w, b, _, dy = make((1, 20, 8), F32, False)
     leaf = x.clone().requires_grad_()
