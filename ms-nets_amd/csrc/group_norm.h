@@ -218,8 +218,9 @@ constexpr int tile_rows(int V, int bytes) { return V * bytes == 16 ? 4 : 8; }
 // Whether a result goes past the caches, and an input that is read for the last time too.  The last-level cache holds 256 MB: a
 // result of an eighth of it and more leaves there as a block of dirty lines that the next pass has to push out before it can keep
 // what it will read again.  Forward and backward of 94 MB: 222 us through the caches, 203 past them; of 805 MB: 1156 and 1113.
-// A smaller result is worth more to whoever reads it next.
-inline bool streams(double bytes) { return bytes >= 32e6; }
+// A smaller result is worth more to whoever reads it next, and lanes of two or four bytes write lines in parts, which only the caches
+// put together (33 channels of bf16, forward and backward of 120 MB: 349 us past them, 318 through them).
+inline bool streams(double bytes, int lane_bytes) { return bytes >= 32e6 && lane_bytes >= 8; }
 
 int check_shape(const char* what, int dtype, int act, int N, long S, int C, int G, double eps);
 // V may be lowered to 1: groups whose edges fall inside vectors and that are too wide to be cut at a common multiple.

@@ -371,7 +371,7 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     cut_rows(&out, V, kApplyBlocks, tile_rows(V, sizeof(T)), kApplyTiles);
     const long grid2 = (long)out.N * out.nblk * out.chunks;
     LaunchScope ls("group_norm_apply", f.stream, 4.0 * sh.N * m * sh.G, bytes);
-    const auto apply = streams((double)sh.N * m * sh.G * sizeof(T)) ? group_norm_apply<T, V, ACT, true> : group_norm_apply<T, V, ACT, false>;
+    const auto apply = streams((double)sh.N * m * sh.G * sizeof(T), V * sizeof(T)) ? group_norm_apply<T, V, ACT, true> : group_norm_apply<T, V, ACT, false>;
     hipLaunchKernelGGL(apply, dim3((unsigned)grid2), dim3(kThreads), (kThreads + sh.gpc) * sizeof(double2), f.stream, x, f.xr, f.weight, f.bias, res,
                        f.rr, (T*)f.y, f.yr, f.stats, out, sh.nblk * sh.nsub, part, pivots, 1. / m, f.eps, f.oflag);
     return check_launch("msnet_group_norm");

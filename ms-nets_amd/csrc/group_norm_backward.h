@@ -386,7 +386,7 @@ static int backward_act(const Backward& f, const BackwardPlan& p, void* ws) {
     cut_rows(&out, V, kGradApplyBlocks, tile_rows(V, sizeof(T)), kGradApplyTiles);
     const unsigned grid2 = (unsigned)((long)out.N * out.nblk * out.chunks) + param_blocks;
     LaunchScope ls("group_norm_grad_apply", f.stream, 8.0 * values, values * sizeof(T) * (RES ? 5 : 3));
-    const auto apply = streams(values * sizeof(T)) ? group_norm_grad_apply<T, V, WHOLE, ACT, RES, true> : group_norm_grad_apply<T, V, WHOLE, ACT, RES, false>;
+    const auto apply = streams(values * sizeof(T), V * sizeof(T)) ? group_norm_grad_apply<T, V, WHOLE, ACT, RES, true> : group_norm_grad_apply<T, V, WHOLE, ACT, RES, false>;
     hipLaunchKernelGGL(apply, dim3(grid2), dim3(kThreads), (kThreads + 2 * sh.gpc) * sizeof(double2), f.stream, dy, f.yr, x, f.xr, res, f.rr, f.weight,
                        f.bias, f.stats, dx, dres, f.dweight, f.dbias, out, sh.nblk * sh.nsub, part, chan, (long)sh.N * sh.nblk, (int)param_blocks, 1. / m);
     return check_launch("msnet_group_norm_backward");
