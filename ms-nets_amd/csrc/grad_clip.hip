@@ -298,22 +298,25 @@ static Cut cut(const int64_t* n, int count) {
 // Whether a value would be written that another tensor of the call reads or writes too: workgroups run in any order, so the result
 // would depend on it.  (A tensor scaled in place is its own input.)
 static bool overlapping(const void* const* in, void* const* out, const int64_t* n, const uint8_t* in_types, const uint8_t* out_types, int count) {
-    struct Range { uintptr_t at, end; bool written; };
-    std::vector<Range> r;
-    r.reserve((size_t)count * 2);
+    struct Range { uintptr_t at, end; };
+    std::vector<Range> read, written;
+    read.reserve((size_t)count);
+    written.reserve((size_t)count);
     for (int i = 0; i < count; ++i) {
         if (!n[i]) continue;
         const uintptr_t p = (uintptr_t)in[i], q = (uintptr_t)out[i];
-        if (p != q || in_types[i] != out_types[i]) r.push_back({p, p + (uintptr_t)n[i] * (in_types[i] ? 2 : 4), false});
-        r.push_back({q, q + (uintptr_t)n[i] * (out_types[i] ? 2 : 4), true});
+        if (p != q || in_types[i] != out_types[i]) read.push_back({p, p + (uintptr_t)n[i] * (in_types[i] ? 2 : 4)});
+        written.push_back({q, q + (uintptr_t)n[i] * (out_types[i] ? 2 : 4)});
     }
     const auto before = [](const Range& a, const Range& b) { return a.at < b.at; };
-    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
-    uintptr_t end = 0, written = 0;                         // of what began so far: all, and what is written
-    for (const Range& a : r) {
-        if (a.at < written || (a.written && a.at < end)) return true;
-        end = std::max(end, a.end);
-        if (a.written) written = std::max(written, a.end);
+    for (auto* r : {&read, &written})                       // (views into one buffer come in order)
+        if (!std::is_sorted(r->begin(), r->end(), before)) std::sort(r->begin(), r->end(), before);
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].at < written[i - 1].end) return true;
+    size_t k = 0;                                           // the first written range that ends behind the one read
+    for (const Range& a : read) {
+        while (k < written.size() && written[k].end <= a.at) ++k;
+        if (k < written.size() && written[k].at < a.end) return true;
     }
     return false;
 }

@@ -212,14 +212,14 @@ PyObject* clip(PyObject*, PyObject* args) {
     const bool write = outs != Py_None, grad = c10::GradMode::is_enabled();
     const Py_ssize_t n = PyList_GET_SIZE(list);
     if (n > INT32_MAX || (write && (!PyList_Check(outs) || PyList_GET_SIZE(outs) != n))) Py_RETURN_NONE;
-    for (Py_ssize_t i = 0; i < n; ++i)                     // (a list of host tensors must not initialise the GPU)
-        if (!THPVariable_Check(PyList_GET_ITEM(list, i)) || !THPVariable_Unpack(PyList_GET_ITEM(list, i)).is_cuda()) Py_RETURN_NONE;
+    if (n && (!THPVariable_Check(PyList_GET_ITEM(list, 0)) || !THPVariable_Unpack(PyList_GET_ITEM(list, 0)).is_cuda())) Py_RETURN_NONE;      // (nothing to ask the GPU)
     const auto device = c10::hip::current_device();
     std::vector<const void*> in(n);
     std::vector<void*> out(write ? n : 0);
     std::vector<int64_t> lengths(n);
     std::vector<uint8_t> types(n), out_types(write ? n : 0);
     for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!THPVariable_Check(PyList_GET_ITEM(list, i))) Py_RETURN_NONE;
         const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
         if (!ordinary(t, device) || !t.is_contiguous()) Py_RETURN_NONE;
         in[i] = t.const_data_ptr();
