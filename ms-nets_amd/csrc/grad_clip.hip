@@ -20,7 +20,7 @@ constexpr int kThreads = 256;
 constexpr int kTensors = 176;          // in a kernel's arguments, which are 4 KB at most
 constexpr int kPart = 216;             // of one launch that writes them to the workspace
 constexpr int kChunk = 16384;          // values of a chunk
-constexpr unsigned kBlocks = 512;      // workgroups at most, all on the device at once (512 MB into 1 GB: 415 us, of 1024 421)
+constexpr unsigned kBlocks = 512;      // workgroups at most, all on the device at once (1024: 2 % slower on 512 MB)
 
 // One tensor.  n: its length, its input's type in bits 44 and 45, its output's in bits 46 and 47.
 struct Entry { const void* in; void* out; unsigned long n; };
@@ -210,9 +210,17 @@ __global__ __launch_bounds__(kThreads) void grad_total(const double* __restrict_
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// Vectors of 16 bytes of the output, so that a wave writes whole lines.
+// A chunk of out = in * f in vectors of 16 bytes of the output, and shifted so that a wave writes whole lines: views into a buffer
+// begin anywhere, and the first chunk takes what lies before its first line too.
 template <bool STREAM, class T, class O>
-__device__ __forceinline__ void scale(const T* p, O* o, int n, float f, int tid) {
+__device__ __forceinline__ void scale(const void* in, void* out, long at, long all, float f, int tid) {
+    const T* p = static_cast<const T*>(in);
+    O* o = static_cast<O*>(out);
+    const int head = (int)min(all, (long)((128 - ((uintptr_t)o & 127)) % 128 / sizeof(O)));
+    if (at == 0 && tid < head) o[tid] = (O)((float)p[tid] * f);
+    p += at + head;
+    o += at + head;
+    const int n = (int)max(0l, min((long)kChunk, all - at - head));
     constexpr int V = 16 / sizeof(O), U = sizeof(T) < sizeof(O) ? 8 : 4;
     typedef typename Pack<T, V>::type Vec;
     typedef typename Pack<O, V>::type Out;
@@ -240,8 +248,8 @@ __device__ __forceinline__ void scale(const T* p, O* o, int n, float f, int tid)
         for (int u = 0; u < U; ++u) put(i + u * kThreads, a[u]);
     }
     for (; i < nv; i += kThreads) put(i, get(i));
-    const int at = nv * V + tid;
-    if (at < n) o[at] = (O)((float)p[at] * f);
+    const int rest = nv * V + tid;
+    if (rest < n) o[rest] = (O)((float)p[rest] * f);
 }
 
 // STREAM: past the caches, for gradients that do not fit them anyway.
@@ -260,15 +268,13 @@ __global__ __launch_bounds__(kThreads) void grad_scale(Source src, unsigned chun
         long at;
         const Entry e = table.find(c, &at);
         if (f != 1.f || e.in != e.out) {                   // (else: short enough already, in place)
-            const int n = (int)min((long)kChunk, length(e) - at);
-            const void* p = e.in;
-            void* o = e.out;
+            const long all = length(e);
             switch (types(e)) {
-                case 0: scale<STREAM>(static_cast<const float*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 1: scale<STREAM>(static_cast<const _Float16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 2: scale<STREAM>(static_cast<const __bf16*>(p) + at, static_cast<float*>(o) + at, n, f, tid); break;
-                case 5: scale<STREAM>(static_cast<const _Float16*>(p) + at, static_cast<_Float16*>(o) + at, n, f, tid); break;
-                default: scale<STREAM>(static_cast<const __bf16*>(p) + at, static_cast<__bf16*>(o) + at, n, f, tid);
+                case 0: scale<STREAM, float, float>(e.in, e.out, at, all, f, tid); break;
+                case 1: scale<STREAM, _Float16, float>(e.in, e.out, at, all, f, tid); break;
+                case 2: scale<STREAM, __bf16, float>(e.in, e.out, at, all, f, tid); break;
+                case 5: scale<STREAM, _Float16, _Float16>(e.in, e.out, at, all, f, tid); break;
+                default: scale<STREAM, __bf16, __bf16>(e.in, e.out, at, all, f, tid);
             }
         }
         if (c < gridDim.x) break;
