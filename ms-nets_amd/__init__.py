@@ -11,6 +11,8 @@ Sub-modules mirror the reference's surfaces:
     libmatchers, libfeatextract                                             (src/cpp/lib/*)
     cbmv_generator.get_costs / extract_features_left / build_ms_volume       (src/dataloader/cbmv_generator.py)
     dist.shard_indices / gather_disparities                                    (replaces nn.DataParallel)
+Beside them, for networks trained on one or two pairs per GPU (not in the reference): hipops.group_norm with its gradient,
+hipops.clip_grads and driver_utils.clip_grad_norm_.
 """
 from . import _lib  # noqa: F401
 
