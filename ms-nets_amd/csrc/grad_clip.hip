@@ -130,9 +130,15 @@ __global__ __launch_bounds__(kThreads) void grad_table(Part p, int at, unsigned 
     begin[tid + 1] = before + sum;
     if (tid == 0) begin[0] = before;
     __syncthreads();
-    if (tid < q.count) { e[at + tid] = mine; first[at + tid] = begin[tid]; }
-    for (int i = tid >> 6; i < q.count; i += kThreads / 64)
-        for (unsigned b = begin[i] + lane; b < begin[i + 1]; b += 64) tensor[b] = (unsigned)(at + i);
+    const bool writes = blockIdx.x == 0;                   // (every workgroup knows all; the first one writes what is short)
+    if (writes && tid < q.count) { e[at + tid] = mine; first[at + tid] = begin[tid]; }
+    if (writes && chunks <= 8)                             // a thread its own; a wave together for those of many, the workgroups in turn
+        for (unsigned b = 0; b < chunks; ++b) tensor[begin[tid] + b] = (unsigned)(at + tid);
+    for (unsigned long many = __ballot(chunks > 8); many; many &= many - 1) {
+        const int i = (tid & ~63) + __builtin_ctzl(many);
+        if (i % gridDim.x == blockIdx.x)
+            for (unsigned b = begin[i] + lane; b < begin[i + 1]; b += 64) tensor[b] = (unsigned)(at + i);
+    }
 }
 
 template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };      // any view's alignment
@@ -420,7 +426,7 @@ extern "C" int msnet_clip_grads(const void* const* in_host, void* const* out_hos
                 next += (unsigned)clip::chunks_of_length(n_host[i]);
             }
             if (p.count == clip::kPart || (i == count - 1 && p.count)) {
-                hipLaunchKernelGGL(clip::grad_table, dim3(1), dim3(clip::kThreads), 0, s, p, at, before, e, first, tensor);
+                hipLaunchKernelGGL(clip::grad_table, dim3(8), dim3(clip::kThreads), 0, s, p, at, before, e, first, tensor);
                 at += p.count;
                 before = next;
                 p.count = 0;

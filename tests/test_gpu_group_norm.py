@@ -207,6 +207,41 @@ def test_another_stream_and_two_at_once(gpu):
         assert torch.equal(y, want[i % 4])
 
 
+@pytest.mark.parametrize("shape,groups", [((70_001, 3, 8), 2), ((70_001, 64), 4), ((1, 2_000_003, 4), 1)])
+def test_very_many_samples_or_rows(gpu, shape, groups):
+    x, w, b, r, dy = make(shape, BF16, True)
+    run_and_check(x, groups, w, b, r, dy, "relu")
+
+
+def test_two_threads(gpu):
+    """Two Python threads, a stream each, forward and backward at once."""
+    import threading
+    sets = [make((1, 20000, 32), F32, True, seed=s) for s in range(2)]
+
+    def step(k):
+        leaves = [t.detach().requires_grad_() for t in sets[k][:4]]
+        y = hipops.group_norm(leaves[0], 8, leaves[1], leaves[2], act="silu", residual=leaves[3])
+        return [y.detach(), *torch.autograd.grad(y, leaves, sets[k][4])]
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    got, errors = {0: [], 1: []}, []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k].append(step(k))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                 # noqa: BLE001  (raised again below, on the test's own thread)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    [t.start() for t in threads]
+    [t.join(60) for t in threads]
+    assert not errors, errors
+    for k in (0, 1):
+        assert len(got[k]) == 20 and all(torch.equal(a, c) for one in got[k] for a, c in zip(one, want[k]))
+
+
 @pytest.mark.parametrize("shape", [(2, 60, 32), (2, 12000, 32)])
 def test_captured_and_replayed(gpu, shape):
     x, w, b, r, dy = make(shape, F32, True)
