@@ -219,7 +219,8 @@ __global__ __launch_bounds__(kThreads) void group_norm_apply(const T* x, Rows xr
     if (oflag && amax >= 0x46ffe000u) atomicOr(oflag, 1u);            // |y| >= 32752, inf or NaN: as the convs' epilogues
 }
 
-// M: vectors a thread holds.  A workgroup takes all rows of one chunk of one sample.
+// M: vectors a thread holds.  A workgroup takes all rows of one chunk of one sample; of sh.nblk workgroups that share one (M / 4 or 1)
+// each writes its part of them.
 template <class T, int V, int M, int ACT>
 __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, const float* __restrict__ weight, const float* __restrict__ bias,
                                                          const T* residual, Rows rr, T* y, Rows yr, double2* __restrict__ stats, Shape sh,
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
     sum_groups(tab, (whole ? cv : k.cw) / k.ng, k.ng, tid, threads, [](int, double2 u) { return u; }, [&](int g, double2 sum) {
         const double2 t = statistics(sum, st[g].x, inv, eps);
         st[g] = t;
-        if (stats) stats[(size_t)k.n * sh.G + k.g0 + g] = t;
+        if (stats && k.blk == 0) stats[(size_t)k.n * sh.G + k.g0 + g] = t;
     });
     __syncthreads();                                       // statistics are there, and nobody reads x any more (y may be x)
     if (!on) return;
@@ -265,6 +266,7 @@ __global__ __launch_bounds__(1024) void group_norm_small(const T* x, Rows xr, co
     unsigned amax = 0u;
 #pragma unroll
     for (int i0 = 0; i0 < M; i0 += 4) {
+        if (sh.nblk > 1 && i0 != 4 * k.blk) continue;
         typename Pack<T, V>::type w[4];
         if (has_res) {
 #pragma unroll
@@ -306,9 +308,10 @@ static int small_threads(const Shape& s, int V, int* M) {
     return 0;
 }
 
-// Chunks of 64 bytes a row (half a cache line) give the single launch the most workgroups; wider ones once those fill the device.
-static Shape small_shape(int N, long S, int C, int G, int* V, int dtype) {
-    long w = 64 / element_bytes(dtype);
+// Chunks of eight channels (or one group) give the single launch the most workgroups and let the longest samples fit: 3060 rows of 32
+// channels of bf16 take 9.5 us with their launch, of 16 channels 11.6, of two launches 17.4.  Wider ones once those fill the device.
+static Shape small_shape(int N, long S, int C, int G, int* V) {
+    long w = 8;
     Shape s = make_shape(N, S, C, G, V, w);
     while ((long)N * s.chunks > 2048 && w < (long)kThreads * *V) {
         w *= 2;
@@ -331,7 +334,7 @@ struct Plan {
 static Plan plan_forward(int N, long S, int C, int G, int dtype) {
     Plan p = {};
     p.V = vector_width(C);
-    p.shape = small_shape(N, S, C, G, &p.V, dtype);
+    p.shape = small_shape(N, S, C, G, &p.V);
     p.threads = p.shape.nsub > 1 ? 0 : small_threads(p.shape, p.V, &p.M);
     if (!p.threads) {
         p.V = vector_width(C);
@@ -350,14 +353,19 @@ static int forward_act(const Forward& f, const Plan& p, void* ws, double bytes) 
     const long grid = (long)sh.N * sh.nblk * sh.chunks;
     const size_t per_table = (sh.cg % V == 0 ? 1 : V) * sizeof(double2);
     if (p.threads) {
+        Shape cut = sh;
+        // Few long chunks: four workgroups a chunk read it and form its statistics, and each writes a quarter (6x17x30x128 in fp32: 8.9 us
+        // for 10.5).  Not in place: one would write what another still reads.
+        if (p.M == 16 && f.x != f.y && (long)sh.N * sh.chunks <= 64) cut.nblk = 4;
+        const dim3 blocks((unsigned)((long)cut.N * cut.nblk * cut.chunks));
         const size_t lds = p.threads * per_table + sh.gpc * sizeof(double2);
         LaunchScope ls("group_norm_small", f.stream, 8.0 * sh.N * m * sh.G, bytes);
         if (p.M == 4)
-            hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
-                               res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+            hipLaunchKernelGGL((group_norm_small<T, V, 4, ACT>), blocks, dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                               res, f.rr, (T*)f.y, f.yr, f.stats, cut, 1. / m, f.eps, f.oflag);
         else
-            hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), dim3((unsigned)grid), dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
-                               res, f.rr, (T*)f.y, f.yr, f.stats, sh, 1. / m, f.eps, f.oflag);
+            hipLaunchKernelGGL((group_norm_small<T, V, 16, ACT>), blocks, dim3(p.threads), lds, f.stream, x, f.xr, f.weight, f.bias,
+                               res, f.rr, (T*)f.y, f.yr, f.stats, cut, 1. / m, f.eps, f.oflag);
         return check_launch("msnet_group_norm");
     }
     double2* part = (double2*)ws;

@@ -17,7 +17,7 @@ static int grad_small_threads(const Shape& s, int V, int dtype, int* M) {
 
 BackwardPlan plan_backward(int N, long S, int C, int G, int dtype) {
     BackwardPlan p = {};
-    long w = 64 / element_bytes(dtype);                     // 64-byte row segments, wider ones once workgroups abound (as in the forward)
+    long w = 8;                                            // as in the forward: narrow chunks, wider ones once workgroups abound
     p.V = vector_width(C);
     p.shape = make_shape(N, S, C, G, &p.V, w);
     while ((long)N * p.shape.chunks > 2048 && w < (long)kThreads * p.V) {
