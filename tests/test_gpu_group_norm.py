@@ -148,6 +148,19 @@ def test_out(gpu, shape):
     assert torch.equal(xx, want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 3060, 128), (2, 4097, 32), (1, 2049, 64)])
+def test_in_place_and_out_of_place_agree(gpu, shape, dtype):
+    """Long chunks: out of place, workgroups share one and each writes its part; in place one writes all of it."""
+    x, w, b, r, _ = make(shape, dtype, True)
+    want = norm64(x, 8, w, b, 1e-5, "relu", r)["y"]
+    y = hipops.group_norm(x, 8, w, b, act="relu", residual=r)
+    within(y, want, "y")
+    for k, out in enumerate((x.clone(), r.clone())):
+        hipops.group_norm(x if k else out, 8, w, b, act="relu", residual=out if k else r, out=out)
+        assert torch.equal(out, y)
+
+
 def test_gradients_against_differences(gpu):
     """d/dt of sum(y * dy) along random directions, by central differences of the operator itself: y is float32, so with step h the
     quotient is off by about |y dy| sqrt(n) 2^-24 / h and h^2 |third derivative| / 6."""
