@@ -248,8 +248,9 @@ int    msnet_group_norm(const void* x, const float* weight, const float* bias, c
                         int dtype, int act, int N, long S, int C, int G, double eps, long x_sn, long x_ss, long r_sn, long r_ss,
                         long y_sn, long y_ss, void* workspace, size_t workspace_bytes, msnet_stream_t stream);
 /* Its gradients from dy and what the forward had (stats included).  dx, dresidual: dense [N][S][C]; dweight, dbias: f32[C]; each
- * may be NULL.  dresidual only with an activation (without one it is dy itself).  The derivative of the ReLU at 0 is 0; on which
- * side of it a value lies is decided in 64 bits.  N or S zero: dweight and dbias become zero. */
+ * may be NULL.  dresidual only with an activation (without one it is dy itself).  The derivative of the ReLU is 0 at 0 and 1 at a
+ * NaN, which the forward passes on too; on which side of 0 a value lies is decided in 64 bits.  N or S zero: dweight and dbias
+ * become zero. */
 size_t msnet_group_norm_backward_workspace_bytes(int dtype, int N, long S, int C, int G);
 int    msnet_group_norm_backward(const void* dy, const void* x, const float* weight, const float* bias, const void* residual,
                                  const double* stats, void* dx, void* dresidual, float* dweight, float* dbias, int dtype, int act,

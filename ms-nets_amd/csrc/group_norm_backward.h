@@ -95,12 +95,12 @@ __device__ __forceinline__ void derive(const Channels<V, WHOLE>& k, const double
                 const double2 t = st[c / cg];
                 double d = ((double)element<T, V>(x, e) - t.x) * t.y * (double)g + (double)b;
                 if constexpr (RES) d += (double)element<T, V>(res, e);
-                z[e] = d > 0. ? 1.f : 0.f;
+                z[e] = d <= 0. ? 0.f : 1.f;
             }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const float g = element<T, V>(dy, e);
-        if constexpr (ACT == kRelu) dz[e] = z[e] > 0.f ? g : 0.f;
+        if constexpr (ACT == kRelu) dz[e] = z[e] <= 0.f ? 0.f : g;       // (a NaN passed the forward, and its gradient passes too)
         else if constexpr (ACT == kSilu) {
             const float sig = silu_gate(z[e]);
             dz[e] = g * (sig * fmaf(z[e], 1.f - sig, 1.f));

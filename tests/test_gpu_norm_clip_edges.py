@@ -1,0 +1,103 @@
+"""hipops.group_norm, grad_norm and clip_grads on the GPU at values, views and calls off the ordinary path: each is answered as the
+definition has it, or refused."""
+import pytest
+import torch
+
+import msnets_amd  # noqa: F401
+from msnets_amd import hipops
+from norm_clip_reference import U, norm64, within
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+NAN, INF = float("nan"), float("inf")
+
+
+def make(shape, dtype, residual, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)              # noqa: E731
+    c = shape[-1]
+    x = (rnd(*shape) * (0.5 + torch.rand(c, device="cuda", generator=g)) + rnd(c)).to(dtype)
+    return x, 1 + 0.3 * rnd(c), 0.3 * rnd(c), rnd(*shape).clamp_min(0).to(dtype) if residual else None, rnd(*shape).to(dtype)
+
+
+def gradients(x, groups, w, b, r, dy, act):
+    leaves = {k: t.detach().clone().requires_grad_() for k, t in zip(("x", "weight", "bias", "residual"), (x, w, b, r)) if t is not None}
+    y = hipops.group_norm(leaves["x"], groups, leaves["weight"], leaves["bias"], act=act, residual=leaves.get("residual"))
+    return {"d" + k: v for k, v in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy))}
+
+
+# ---- what is not finite, backward: in one launch and in two ---------------------------------------------------------------
+
+BOTH_WAYS = [(2, 60, 16), (2, 30000, 16)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("shape", BOTH_WAYS)
+def test_relu_gradient_at_nonfinite_residuals(gpu, shape, dtype):
+    """A NaN passes the ReLU and so does its gradient; +inf passes it, -inf does not.  All gradients stay finite: they are those of
+    a residual with +1000 and -1000 in these places."""
+    x, w, b, r, dy = make(shape, dtype, True)
+    r[1, 7, 5], r[0, 0, 1], r[1, 8, 5], r[0, 3, 2] = NAN, NAN, INF, -INF
+    want = norm64(x, 4, w, b, 1e-5, "relu", r.nan_to_num(nan=1000.0, posinf=1000.0, neginf=-1000.0), dy)
+    for k, v in gradients(x, 4, w, b, r, dy, "relu").items():
+        within(v, want[k], k)
+
+
+@pytest.mark.parametrize("where", [0, 7])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("shape", BOTH_WAYS)
+def test_relu_gradient_of_a_nonfinite_group(gpu, shape, bad, where):
+    """Something in x that is not finite makes xhat a NaN in its whole group: dy passes there (dresidual, dbias), dx and dgamma are
+    NaN, and nothing else changes."""
+    x, w, b, r, dy = make(shape, F32, True)
+    lifted = r.clone()
+    lifted[1, :, 4:8] = 1000.0                 # a group that passes everywhere, for dresidual and dbias
+    want, ordinary = norm64(x, 4, w, b, 1e-5, "relu", lifted, dy), norm64(x, 4, w, b, 1e-5, "relu", r, dy)
+    x[1, where, 5] = bad
+    got = gradients(x, 4, w, b, r, dy, "relu")
+    within(got["dresidual"], want["dresidual"], "dresidual")
+    within(got["dbias"], want["dbias"], "dbias")
+    assert torch.isnan(got["dx"][1, :, 4:8]).all() and torch.isnan(got["dweight"][4:8]).all()
+    rest = torch.ones(16, dtype=torch.bool, device="cuda")
+    rest[4:8] = False
+    within(got["dweight"][rest], tuple(t[rest] for t in ordinary["dweight"]), "dweight")
+    for at in ((0,), (1, slice(None), rest)):
+        within(got["dx"][at], tuple(t[at] for t in ordinary["dx"]), "dx")
+
+
+@pytest.mark.parametrize("act", ["relu", "silu"])
+@pytest.mark.parametrize("shape", BOTH_WAYS)
+def test_nonfinite_incoming_gradient(gpu, shape, act):
+    """In dy: its own value in dresidual, its channel's parameters and its group's dx; with a ReLU only where that passes."""
+    x, w, b, r, dy = make(shape, F32, True)
+    z = norm64(x, 4, w, b, 1e-5, "none", r)["y"][0]
+    on = int((z[1, :, 5] > 0.1).nonzero()[0])
+    off = int((z[1, :, 9] < -0.1).nonzero()[0])
+    want = norm64(x, 4, w, b, 1e-5, act, r, dy)
+    clean = dy.clone()
+    clean[1, off, 9] = 0
+    blocked = norm64(x, 4, w, b, 1e-5, act, r, clean)
+    dy[1, on, 5], dy[1, off, 9] = NAN, (INF if act == "relu" else dy[1, off, 9])
+    got = gradients(x, 4, w, b, r, dy, act)
+    assert torch.isnan(got["dresidual"][1, on, 5]) and torch.isnan(got["dweight"][5]) and torch.isnan(got["dbias"][5])
+    assert torch.isnan(got["dx"][1, :, 4:8]).all()
+    ref = blocked if act == "relu" else want
+    rest = torch.ones(16, dtype=torch.bool, device="cuda")
+    rest[4:8] = False
+    for k in ("dweight", "dbias"):
+        within(got[k][rest], tuple(t[rest] for t in ref[k]), k)
+    for k in ("dx", "dresidual"):
+        within(got[k][..., rest], tuple(t[..., rest] for t in ref[k]), k)
+        within(got[k][0], tuple(t[0] for t in ref[k]), k)
+
+
+@pytest.mark.parametrize("shape", BOTH_WAYS)
+def test_silu_of_a_nan(gpu, shape):
+    """SiLU has no side for a NaN to pass on: everything it reaches is one."""
+    x, w, b, r, dy = make(shape, F32, True)
+    want = norm64(x, 4, w, b, 1e-5, "silu", r, dy)
+    r[1, 7, 5] = NAN
+    got = gradients(x, 4, w, b, r, dy, "silu")
+    assert torch.isnan(got["dresidual"][1, 7, 5]) and torch.isnan(got["dx"][1, :, 4:8]).all()
+    within(got["dx"][0], tuple(t[0] for t in want["dx"]), "dx")
+    within(got["dbias"][:4], tuple(t[:4] for t in want["dbias"]), "dbias")
