@@ -296,7 +296,8 @@ int msnet_epe_badx(const float* gt, const float* pred, size_t n, float max_disp,
 /* ---- training-side: the global gradient norm and clipping -------------------------------------- */
 /* norm = sqrt(sum of the squares of all values of all `count` tensors); out = in * min(1, max_norm / (norm + 1e-6)).
  * The four / five arrays are HOST arrays of `count` entries (device pointers, lengths, types 0 float32 / 1 float16 / 2 bfloat16);
- * an output has its input's type or float32, and may be the input itself.  out_host = NULL: the norm alone.  norm: device f32.
+ * an output has its input's type or float32, and may be the input itself.  out_host = NULL: the norm alone.  norm: device f32,
+ * infinite where float32 cannot hold it (the factor is formed from the 64-bit norm).
  * An infinite norm scales every finite value to 0 and a NaN makes every value one: nothing is checked on the host.  Outputs that
  * overlap anything else of the call are refused.  workspace: msnet_clip_grads_workspace_bytes() bytes, 8-byte aligned. */
 size_t msnet_clip_grads_workspace_bytes(const int64_t* n_host, int count);

@@ -605,7 +605,7 @@ def _grad_list(grads):
 
 def grad_norm(grads):
     """The 2-norm over all values of all the given tensors (float32, float16, bfloat16, any shapes and mix): a float32 scalar on the
-    device, nothing waits for it.  Squares are formed and added in 64 bits."""
+    device, nothing waits for it.  Squares are formed and added in 64 bits; a norm past float32's range is returned as infinity."""
     grads = _grad_list(grads)
     host = _lib.load_host()
     norm = host.clip(grads, None, 0.0)

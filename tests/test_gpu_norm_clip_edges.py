@@ -101,3 +101,26 @@ def test_silu_of_a_nan(gpu, shape):
     assert torch.isnan(got["dresidual"][1, 7, 5]) and torch.isnan(got["dx"][1, :, 4:8]).all()
     within(got["dx"][0], tuple(t[0] for t in want["dx"]), "dx")
     within(got["dbias"][:4], tuple(t[:4] for t in want["dbias"]), "dbias")
+
+
+# ---- clipping: gradients at the ends of their types' range -----------------------------------------------------------------
+
+@pytest.mark.parametrize("max_norm", [1e3, 1e-3, 1e-30])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_factors_below_float32s_normal_range(gpu, dtype, max_norm):
+    """Gradients near the largest float: max_norm / norm is next to 2^-126 (1e3) or below it, where a float32 has fewer bits the smaller
+    it is.  The factor and the products round by half a step each, as for any other factor; results below 2^-126 by half of the last step more."""
+    values = [1e38, -3e38, 2.5e37, 1e30, -1e20, 1.0, 1e-20, 0.0]
+    t = torch.tensor(values * 4000, device="cuda").to(dtype)
+    short = t[:13].clone()
+    norm = (t.double().square().sum() + short.double().square().sum()).sqrt()
+    assert float(norm) > torch.finfo(F32).max
+    before = [t.clone(), short.clone()]
+    out = [torch.empty_like(t, dtype=F32), torch.empty_like(short, dtype=F32)]
+    assert float(hipops.clip_grads([t, short], max_norm, out=out)) == INF
+    hipops.clip_grads([t, short], max_norm)
+    for got in (out, [t, short]):
+        for v, o in zip(before, got):
+            want = v.double() * (max_norm / (float(norm) + 1e-6))
+            allowed = 2.1 * U * want.abs() + torch.finfo(o.dtype).eps / 2 * want.abs() * (1 + 3 * U) + 2.0 ** -149 + (2.0 ** -134 if o.dtype == BF16 else 0)
+            assert bool(((o.double() - want).abs() <= allowed).all())
