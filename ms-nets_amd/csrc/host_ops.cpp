@@ -36,7 +36,7 @@ void succeed(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed: ",
 int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1; }
 
 bool ordinary(const Tensor& t, c10::DeviceIndex device) {
-    return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && type_code(t.scalar_type()) >= 0;
+    return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && type_code(t.scalar_type()) >= 0 && !t.is_neg();
 }
 
 void* stream_of(c10::DeviceIndex device) { return c10::hip::getCurrentHIPStream(device).stream(); }
@@ -127,7 +127,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         torch::autograd::variable_list out(7);
         {
             c10::AutoGradMode off(false);
-            Tensor dy = grads[0];
+            Tensor dy = grads[0].resolve_neg();            // (a view with its sign bit to be applied is none the kernels can read)
             Rows yr, xr, rr;
             if (!rows_of(dy, &yr)) {
                 dy = dy.contiguous();

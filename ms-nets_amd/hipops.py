@@ -546,8 +546,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
             return y
     _check_norm_args(x, groups, weight, bias, eps, act, residual)       # something to refuse, to lay out or to place
     groups, eps = int(groups), float(eps)
-    plain = lambda p: p if p is None or (p.dtype == torch.float32 and p.is_contiguous()) else p.float().contiguous()      # noqa: E731
-    even = lambda t: t if t is None or _row_strides(t) is not None else t.contiguous()                                    # noqa: E731
+    plain = lambda p: p if p is None else p.float().contiguous().resolve_neg()                                            # noqa: E731
+    even = lambda t: t if t is None else (t if _row_strides(t) is not None else t.contiguous()).resolve_neg()             # noqa: E731
     x, residual, weight, bias = even(x), even(residual), plain(weight), plain(bias)
     graded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
     if graded and out is not None:
@@ -568,6 +568,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
             raise ValueError("out must be %s %s with consecutive channels and evenly spaced rows of its own" % (x.dtype, tuple(x.shape)))
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("out must not require a gradient")
+        if out.is_neg():
+            raise ValueError("out must not be a negated view")
         _check_out(out, x, "x")
         _check_out(out, residual, "residual")
     lib, code, xs, ys, rs = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(out), _row_strides(residual) if residual is not None else (0, 0)
@@ -612,7 +614,7 @@ def grad_norm(grads):
     if norm is None:                                        # something to refuse, or to lay out
         for i, t in enumerate(grads):
             _require_gpu(t, "grads[%d]" % i)
-        norm = host.clip([_flat(t) if _is_dense(t) else t.detach().contiguous() for t in grads], None, 0.0)
+        norm = host.clip([_flat(t) if _is_dense(t) and not t.is_neg() else t.detach().contiguous().resolve_neg() for t in grads], None, 0.0)
     return norm
 
 
@@ -654,11 +656,11 @@ def _clip_layout(grads, outs):
         if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
             raise ValueError("a tensor to be written is expanded: its values share memory")
         t, o = t.detach(), o.detach()
-        if _is_dense(t) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())):
+        if not t.is_neg() and not o.is_neg() and _is_dense(t) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())):
             src.append(_flat(t))                            # a value has the same place in memory on both sides
             dst.append(_flat(o))
         else:
-            src.append(t.contiguous().view(-1))
+            src.append(t.contiguous().resolve_neg().view(-1))
             dst.append(torch.empty(src[-1].shape, device=o.device, dtype=o.dtype))
             back.append((o, dst[-1].view(o.shape)))
     return src, dst, back

@@ -124,3 +124,44 @@ def test_factors_below_float32s_normal_range(gpu, dtype, max_norm):
             want = v.double() * (max_norm / (float(norm) + 1e-6))
             allowed = 2.1 * U * want.abs() + torch.finfo(o.dtype).eps / 2 * want.abs() * (1 + 3 * U) + 2.0 ** -149 + (2.0 ** -134 if o.dtype == BF16 else 0)
             assert bool(((o.double() - want).abs() <= allowed).all())
+
+
+# ---- negated views: what .conj().imag of a complex tensor is -----------------------------------------------------------------
+
+def negated(t):
+    """t's values as a view whose memory holds their negatives, laid out as t is."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_group_norm_of_negated_views(gpu):
+    x, w, b, r, dy = make((2, 50, 16), F32, True)
+    want = gradients(x, 4, w, b, r, dy, "silu")
+    y = hipops.group_norm(x, 4, w, b, act="silu", residual=r)
+    for i in range(4):
+        args = [negated(t) if k == i else t for k, t in enumerate((x, w, b, r))]
+        assert torch.equal(hipops.group_norm(args[0], 4, args[1], args[2], act="silu", residual=args[3]), y), i
+        assert torch.equal(hipops.group_norm(args[0], 4, args[1], args[2], act="silu", residual=args[3], out=torch.empty_like(x)), y), i
+        got = [t.requires_grad_() for t in args]
+        got = torch.autograd.grad(hipops.group_norm(got[0], 4, got[1], got[2], act="silu", residual=got[3]), got, negated(dy))
+        assert all(torch.equal(a, c) for a, c in zip(got, want.values())), i
+        for t in (x, w, b, r):
+            t.requires_grad_(False)
+    with pytest.raises(ValueError, match="negated"):
+        hipops.group_norm(x, 4, w, b, out=negated(x))
+    z = torch.complex(x, -x).conj().imag[..., :1]                # (a stride of two floats, a negated one)
+    assert z.is_neg() and torch.equal(hipops.group_norm(z, 1), hipops.group_norm(z.resolve_neg(), 1))
+
+
+def test_clipping_of_negated_views(gpu):
+    a, c = make((40, 8), F32, False)[0], make((7,), F32, False, seed=1)[0]
+    want = [torch.empty_like(a), torch.empty_like(c)]
+    norm = hipops.clip_grads([a, c], 1.0, out=want)
+    na, nc = negated(a), negated(c)
+    out = [torch.empty_like(a), torch.empty_like(c)]
+    assert torch.equal(hipops.clip_grads([na, c], 1.0, out=out), norm) and all(torch.equal(p, q) for p, q in zip(out, want))
+    out = [negated(a), negated(c)]
+    assert torch.equal(hipops.clip_grads([a, nc], 1.0, out=out), norm) and all(torch.equal(p, q) for p, q in zip(out, want))
+    assert torch.equal(hipops.grad_norm([na, nc]), norm)
+    assert torch.equal(hipops.clip_grads([na, nc], 1.0), norm) and torch.equal(na, want[0]) and torch.equal(nc, want[1])
