@@ -5,15 +5,18 @@
 //
 // An operator takes ordinary arguments and returns None for all others: hipops.py then lays the tensors out, or says what is wrong.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <vector>
 
@@ -37,6 +40,15 @@ int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 
 
 bool ordinary(const Tensor& t, c10::DeviceIndex device) {
     return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && type_code(t.scalar_type()) >= 0 && !t.is_neg();
+}
+
+// Forward-mode tangents are not carried on: a result without one would stand for a derivative of zero.  A call asks once whether any
+// can exist (asking 1000 views and their outputs one by one took 45 us).
+bool tangents_exist() { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0); }
+
+void refuse_tangent(const Tensor& t, const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what,
+                                " has no forward-mode derivative (use reverse mode, or hand it tensors without a tangent)");
 }
 
 void* stream_of(c10::DeviceIndex device) { return c10::hip::getCurrentHIPStream(device).stream(); }
@@ -181,6 +193,8 @@ PyObject* group_norm(PyObject*, PyObject* args) {
     Tensor x, w, b, r;
     if (!tensor_or_none(px, &x) || !x.defined() || !tensor_or_none(pw, &w) || !tensor_or_none(pb, &b) || !tensor_or_none(pr, &r) || !x.is_cuda())
         Py_RETURN_NONE;
+    if (tangents_exist())
+        for (const Tensor* t : {&x, &w, &b, &r}) refuse_tangent(*t, "group_norm");
     const auto device = c10::hip::current_device();
     Rows any;
     if (!ordinary(x, device) || x.dim() < 2 || !rows_of(x, &any) || x.size(-1) < 1 || groups < 1 || x.size(-1) % groups || !(eps >= 0.) || eps > 1e300 ||
@@ -209,7 +223,7 @@ PyObject* clip(PyObject*, PyObject* args) {
     PyObject *list, *outs;
     double max_norm;
     if (!PyArg_ParseTuple(args, "O!Od", &PyList_Type, &list, &outs, &max_norm)) return nullptr;
-    const bool write = outs != Py_None, grad = c10::GradMode::is_enabled();
+    const bool write = outs != Py_None, grad = c10::GradMode::is_enabled(), tangents = tangents_exist();
     const Py_ssize_t n = PyList_GET_SIZE(list);
     if (n > INT32_MAX || (write && (!PyList_Check(outs) || PyList_GET_SIZE(outs) != n))) Py_RETURN_NONE;
     if (n && (!THPVariable_Check(PyList_GET_ITEM(list, 0)) || !THPVariable_Unpack(PyList_GET_ITEM(list, 0)).is_cuda())) Py_RETURN_NONE;      // (nothing to ask the GPU)
@@ -221,6 +235,7 @@ PyObject* clip(PyObject*, PyObject* args) {
     for (Py_ssize_t i = 0; i < n; ++i) {
         if (!THPVariable_Check(PyList_GET_ITEM(list, i))) Py_RETURN_NONE;
         const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+        if (tangents) refuse_tangent(t, write ? "clip_grads" : "grad_norm");
         if (!ordinary(t, device) || !t.is_contiguous()) Py_RETURN_NONE;
         in[i] = t.const_data_ptr();
         lengths[i] = t.numel();
@@ -229,6 +244,7 @@ PyObject* clip(PyObject*, PyObject* args) {
         PyObject* po = PyList_GET_ITEM(outs, i);
         if (!THPVariable_Check(po)) Py_RETURN_NONE;
         const Tensor& o = THPVariable_Unpack(po);
+        if (tangents) refuse_tangent(o, "clip_grads");
         if (!ordinary(o, device) || !o.is_contiguous() || (o.scalar_type() != t.scalar_type() && o.scalar_type() != at::kFloat) ||
             (!o.is_same(t) && o.sizes() != t.sizes()) || (grad && o.requires_grad()))
             Py_RETURN_NONE;
@@ -247,6 +263,21 @@ PyObject* clip(PyObject*, PyObject* args) {
         if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     }
     return THPVariable_Wrap(norm);
+    END_HANDLE_TH_ERRORS
+}
+
+// refuse_tangents(what, tensors): an error if one of them has a tangent (anything else among them is passed over).
+PyObject* refuse_tangents(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    const char* what;
+    PyObject* tensors;
+    if (!PyArg_ParseTuple(args, "sO", &what, &tensors)) return nullptr;
+    const THPObjectPtr items(PySequence_Fast(tensors, "refuse_tangents() takes a sequence"));
+    if (!items) return nullptr;
+    if (!tangents_exist()) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.get()); ++i)
+        if (PyObject* o = PySequence_Fast_GET_ITEM(items.get(), i); THPVariable_Check(o)) refuse_tangent(THPVariable_Unpack(o), what);
+    Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
 
@@ -269,6 +300,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 
 PyMethodDef methods[] = {{"bind", bind, METH_O, "bind({name: address})"},
                          {"group_norm", group_norm, METH_VARARGS, "group_norm(x, groups, weight, bias, eps, act, residual)"},
+                         {"refuse_tangents", refuse_tangents, METH_VARARGS, "refuse_tangents(what, tensors)"},
                          {"clip", clip, METH_VARARGS, "clip(tensors, outs, max_norm)"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

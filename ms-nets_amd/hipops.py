@@ -537,14 +537,15 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
     slices of wider tensors are taken as they are, other strides are copied.  out: where the result goes -- x or residual
     themselves, or memory beside them; only where no gradient is asked for.
 
-    With gradients enabled the result is differentiable once in x, weight, bias and residual; x, the residual (with an activation)
-    and 16 bytes a sample and group are kept for it.  Results and gradients repeat bit for bit.  Inside a forward of the aggregators
+    With gradients enabled the result is differentiable once, in reverse mode, in x, weight, bias and residual; x, the residual (with
+    an activation) and 16 bytes a sample and group are kept for it.  Results and gradients repeat bit for bit.  Inside a forward of the aggregators
     the result raises the fp16-range flag as a conv's does (RangeGuard)."""
     if out is None and _tls.arena is None and act in _ACT_CODES and type(groups) is int:
         y = _lib.load_host().group_norm(x, groups, weight, bias, eps, _ACT_CODES[act], residual)
         if y is not None:
             return y
     _check_norm_args(x, groups, weight, bias, eps, act, residual)       # something to refuse, to lay out or to place
+    _lib.load_host().refuse_tangents("group_norm", (x, weight, bias, residual, out))
     groups, eps = int(groups), float(eps)
     plain = lambda p: p if p is None else p.float().contiguous().resolve_neg()                                            # noqa: E731
     even = lambda t: t if t is None else (t if _row_strides(t) is not None else t.contiguous()).resolve_neg()             # noqa: E731
@@ -614,6 +615,7 @@ def grad_norm(grads):
     if norm is None:                                        # something to refuse, or to lay out
         for i, t in enumerate(grads):
             _require_gpu(t, "grads[%d]" % i)
+        host.refuse_tangents("grad_norm", grads)
         norm = host.clip([_flat(t) if _is_dense(t) and not t.is_neg() else t.detach().contiguous().resolve_neg() for t in grads], None, 0.0)
     return norm
 
@@ -631,6 +633,8 @@ def clip_grads(grads, max_norm, out=None):
     host = _lib.load_host()
     norm = host.clip(grads, outs, max_norm)
     if norm is None:
+        host.refuse_tangents("clip_grads", grads)
+        host.refuse_tangents("clip_grads", outs)
         src, dst, back = _clip_layout(grads, outs)
         norm = host.clip(src, dst, max_norm)
         for o, d in back:

@@ -165,3 +165,33 @@ def test_clipping_of_negated_views(gpu):
     assert torch.equal(hipops.clip_grads([a, nc], 1.0, out=out), norm) and all(torch.equal(p, q) for p, q in zip(out, want))
     assert torch.equal(hipops.grad_norm([na, nc]), norm)
     assert torch.equal(hipops.clip_grads([na, nc], 1.0), norm) and torch.equal(na, want[0]) and torch.equal(nc, want[1])
+
+
+# ---- derivatives that the operators do not have are refused, not dropped -----------------------------------------------------
+
+def test_forward_mode_is_refused(gpu):
+    import torch.autograd.forward_ad as forward_ad
+    full = make((2, 60, 16), F32, True)[:4]
+    for base in (full, [full[0][..., :12].transpose(0, 1), full[1][:12].bfloat16(), full[2][:12].half(), full[3][..., :12].transpose(0, 1)]):
+        for i in range(4):
+            with forward_ad.dual_level():
+                args = [forward_ad.make_dual(t, torch.ones_like(t)) if k == i else t for k, t in enumerate(base)]
+                for mode in (torch.enable_grad, torch.no_grad):                   # (tangents do not depend on this mode)
+                    for out in (None, torch.empty_like(base[0], memory_format=torch.contiguous_format)):
+                        with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                            hipops.group_norm(args[0], 4, args[1], args[2], residual=args[3], out=out)
+                hipops.group_norm(*[forward_ad.unpack_dual(args[0]).primal, 4, *base[1:3]])       # nothing is left behind
+    with forward_ad.dual_level():
+        out = forward_ad.make_dual(torch.empty_like(full[0]), full[0])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            hipops.group_norm(full[0], 4, out=out)
+        for t in (full[0], full[0].transpose(0, 1), full[0][:, ::2]):
+            d = forward_ad.make_dual(t, torch.ones_like(t))
+            for call in (lambda: hipops.grad_norm([d]), lambda: hipops.clip_grads([d], 1.0), lambda: hipops.clip_grads([t], 1.0, out=[d]),
+                         lambda: hipops.clip_grads([full[1], d], 1.0, out=[full[1].clone(), torch.empty_like(t)])):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+    for transform in (lambda f, t: torch.func.jvp(f, (t,), (t,)), lambda f, t: torch.func.grad(lambda u: f(u).sum())(t), lambda f, t: torch.func.vmap(f)(t)):
+        for f in (lambda t: hipops.group_norm(t, 4), lambda t: hipops.group_norm(t, 4, out=torch.empty_like(full[0][:1])), lambda t: hipops.grad_norm([t])):
+            with pytest.raises((RuntimeError, ValueError)):
+                transform(f, full[0][None, :1])
