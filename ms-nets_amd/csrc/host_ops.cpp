@@ -217,7 +217,7 @@ PyObject* group_norm(PyObject*, PyObject* args) {
 // ---- gradient clipping -----------------------------------------------------------------------------------------------
 
 // clip(tensors, outs, max_norm): the norm, or None where a tensor is not ordinary (contiguous, of a known type, on the current
-// device; an output of its input's shape, of its type or float32, and without a gradient of its own).  outs None: the norm alone.
+// device, not part of a graph being recorded; an output of its input's shape, and of its type or float32).  outs None: the norm alone.
 PyObject* clip(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
     PyObject *list, *outs;
@@ -236,7 +236,7 @@ PyObject* clip(PyObject*, PyObject* args) {
         if (!THPVariable_Check(PyList_GET_ITEM(list, i))) Py_RETURN_NONE;
         const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
         if (tangents) refuse_tangent(t, write ? "clip_grads" : "grad_norm");
-        if (!ordinary(t, device) || !t.is_contiguous()) Py_RETURN_NONE;
+        if (!ordinary(t, device) || !t.is_contiguous() || (grad && t.requires_grad())) Py_RETURN_NONE;
         in[i] = t.const_data_ptr();
         lengths[i] = t.numel();
         types[i] = (uint8_t)type_code(t.scalar_type());

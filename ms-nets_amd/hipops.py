@@ -606,15 +606,22 @@ def _grad_list(grads):
     return [grads] if isinstance(grads, torch.Tensor) else list(grads)
 
 
+def _refuse_graph(t, name):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient, and the norm and clipping carry none on: detach() it, or call under torch.no_grad()" % name)
+
+
 def grad_norm(grads):
     """The 2-norm over all values of all the given tensors (float32, float16, bfloat16, any shapes and mix): a float32 scalar on the
-    device, nothing waits for it.  Squares are formed and added in 64 bits; a norm past float32's range is returned as infinity."""
+    device, nothing waits for it.  Squares are formed and added in 64 bits; a norm past float32's range is returned as infinity.  No
+    gradient flows through it: tensors that require one are refused outside torch.no_grad()."""
     grads = _grad_list(grads)
     host = _lib.load_host()
     norm = host.clip(grads, None, 0.0)
     if norm is None:                                        # something to refuse, or to lay out
         for i, t in enumerate(grads):
             _require_gpu(t, "grads[%d]" % i)
+            _refuse_graph(t, "grads[%d]" % i)
         host.refuse_tangents("grad_norm", grads)
         norm = host.clip([_flat(t) if _is_dense(t) and not t.is_neg() else t.detach().contiguous().resolve_neg() for t in grads], None, 0.0)
     return norm
@@ -624,7 +631,8 @@ def clip_grads(grads, max_norm, out=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)), norm the 2-norm over all of them (grad_norm), and returns the norm:
     in place, or into `out`, one tensor a gradient of its shape, of its type or float32.  Gradients that are short enough are left
     as they are (in place nothing is written).  The host is never asked: an infinite norm scales finite values to 0, and a NaN among
-    the gradients makes all of them NaN.  A tensor listed twice, or one that overlaps another, is refused where it would be written."""
+    the gradients makes all of them NaN.  A tensor listed twice, or one that overlaps another, is refused where it would be written, and
+    so are tensors that require a gradient, outside torch.no_grad()."""
     grads = _grad_list(grads)
     outs = grads if out is None else _grad_list(out)
     max_norm = float(max_norm)
@@ -659,6 +667,7 @@ def _clip_layout(grads, outs):
             raise ValueError("a tensor to be written requires a gradient itself")
         if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
             raise ValueError("a tensor to be written is expanded: its values share memory")
+        _refuse_graph(t, "grads[%d]" % i)
         t, o = t.detach(), o.detach()
         if not t.is_neg() and not o.is_neg() and _is_dense(t) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())):
             src.append(_flat(t))                            # a value has the same place in memory on both sides

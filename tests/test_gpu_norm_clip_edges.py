@@ -195,3 +195,22 @@ def test_forward_mode_is_refused(gpu):
         for f in (lambda t: hipops.group_norm(t, 4), lambda t: hipops.group_norm(t, 4, out=torch.empty_like(full[0][:1])), lambda t: hipops.grad_norm([t])):
             with pytest.raises((RuntimeError, ValueError)):
                 transform(f, full[0][None, :1])
+
+
+def test_gradients_of_the_norm_are_refused(gpu):
+    """Gradients that carry a graph, as a penalty on their norm would have them; taken as numbers under no_grad."""
+    p = torch.tensor([3.0, 4.0], device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(0.5 * p.square().sum(), p, create_graph=True)
+    column = (p[:, None] * torch.ones(2, 3, device="cuda"))[:, ::2]             # one of other strides
+    for t in (g, p, column):
+        out = torch.full_like(t, 7.0).detach()
+        for call in (lambda: hipops.grad_norm([t]), lambda: hipops.grad_norm(t), lambda: hipops.clip_grads([t], 1.0, out=[out]),
+                     lambda: hipops.clip_grads([out, t], 1.0, out=[out, torch.empty_like(out)])):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call()
+        assert bool((out == 7).all())
+        with torch.no_grad():
+            n = hipops.grad_norm([t])
+            assert torch.equal(n, hipops.clip_grads([t], 1.0, out=[out])) and float(out.norm()) <= 1 + 1e-6
+        assert torch.equal(n, hipops.grad_norm([t.detach()]))
+    hipops.clip_grads([p.detach()], 1.0)
