@@ -110,13 +110,17 @@ Tensor forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const 
 // While a stream is captured, a leaf must not still be held by a graph that was recorded on another stream: its accumulation node
 // belongs to that stream, the captured backward would make the two wait for each other, and torch ends the process there.
 void check_capture(const Tensor& t) {
-    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+    if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) return;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!node) return;
     const auto theirs = node->stream();
     TORCH_CHECK(!theirs || *theirs == c10::hip::getCurrentHIPStream(t.get_device()).unwrap(),
                 "group_norm is being captured while a graph recorded on another stream still holds one of its leaves: drop the results of earlier "
                 "eager steps on these tensors first");
+}
+
+bool recorded_in_capture() {
+    return c10::GradMode::is_enabled() && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
 }
 
 struct GroupNorm : torch::autograd::Function<GroupNorm> {
@@ -206,7 +210,7 @@ PyObject* group_norm(PyObject*, PyObject* args) {
     if (r.defined() && (!ordinary(r, device) || r.scalar_type() != x.scalar_type() || r.sizes() != x.sizes() || !rows_of(r, &any))) Py_RETURN_NONE;
     const bool grad = c10::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()) ||
                                                       (r.defined() && r.requires_grad()));
-    if (grad && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    if (grad && recorded_in_capture())
         for (const Tensor* t : {&x, &w, &b, &r}) check_capture(*t);
     const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     return THPVariable_Wrap(grad ? GroupNorm::apply(x, given(w), given(b), given(r), (int64_t)groups, eps, (int64_t)act)
@@ -281,6 +285,19 @@ PyObject* refuse_tangents(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// refuse_capture(tensors): an error where group_norm is being captured and one of the tensors must not be (check_capture).  For those
+// that are laid out or cast first: what group_norm gets then is no leaf any more, but its graph ends at the same one.
+PyObject* refuse_capture(PyObject*, PyObject* tensors) {
+    HANDLE_TH_ERRORS
+    const THPObjectPtr items(PySequence_Fast(tensors, "refuse_capture() takes a sequence"));
+    if (!items) return nullptr;
+    if (!recorded_in_capture()) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.get()); ++i)
+        if (PyObject* o = PySequence_Fast_GET_ITEM(items.get(), i); THPVariable_Check(o)) check_capture(THPVariable_Unpack(o));
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the library's entry points.
 PyObject* bind(PyObject*, PyObject* table) {
     if (!PyDict_Check(table)) return PyErr_Format(PyExc_TypeError, "bind() takes a dict of addresses");
@@ -301,6 +318,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 PyMethodDef methods[] = {{"bind", bind, METH_O, "bind({name: address})"},
                          {"group_norm", group_norm, METH_VARARGS, "group_norm(x, groups, weight, bias, eps, act, residual)"},
                          {"refuse_tangents", refuse_tangents, METH_VARARGS, "refuse_tangents(what, tensors)"},
+                         {"refuse_capture", refuse_capture, METH_O, "refuse_capture(tensors)"},
                          {"clip", clip, METH_VARARGS, "clip(tensors, outs, max_norm)"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

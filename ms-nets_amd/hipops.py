@@ -546,6 +546,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
             return y
     _check_norm_args(x, groups, weight, bias, eps, act, residual)       # something to refuse, to lay out or to place
     _lib.load_host().refuse_tangents("group_norm", (x, weight, bias, residual, out))
+    _lib.load_host().refuse_capture((x, weight, bias, residual))
     groups, eps = int(groups), float(eps)
     plain = lambda p: p if p is None else p.float().contiguous().resolve_neg()                                            # noqa: E731
     even = lambda t: t if t is None else (t if _row_strides(t) is not None else t.contiguous()).resolve_neg()             # noqa: E731

@@ -214,3 +214,35 @@ def test_gradients_of_the_norm_are_refused(gpu):
             assert torch.equal(n, hipops.clip_grads([t], 1.0, out=[out])) and float(out.norm()) <= 1 + 1e-6
         assert torch.equal(n, hipops.grad_norm([t.detach()]))
     hipops.clip_grads([p.detach()], 1.0)
+
+
+# ---- capture: leaves that are cast or laid out before the kernels see them ---------------------------------------------------
+
+def test_capture_beside_a_live_eager_graph_of_other_types_and_strides(gpu):
+    """A leaf of another type or stride reaches the kernels as a copy whose graph ends at the leaf: its eager graph stands in a captured
+    backward's way as one of a plain leaf does, and the captured forward refuses it likewise."""
+    x, w, b, r, dy = make((2, 60, 16), F32, True)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)                          # noqa: E731
+    for i, leaf in ((0, turned(x)), (1, w.bfloat16()), (1, torch.stack([w, w], 1)[:, 0]), (2, b.half()), (3, turned(r))):
+        leaf = leaf.detach().requires_grad_()
+        args = [leaf if k == i else t for k, t in enumerate((x, w, b, r))]
+        run = lambda: hipops.group_norm(args[0], 4, args[1], args[2], act="relu", residual=args[3])      # noqa: E731,B023
+        alive = run()
+        with pytest.raises(RuntimeError, match="drop the results"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                run()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = run()
+            d, = torch.autograd.grad(y, leaf, dy)
+            y = y.detach()
+        for seed in range(3):
+            with torch.no_grad():
+                leaf.copy_(make((2, 60, 16), F32, True, seed=seed)[i])
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [y.clone(), d.clone()]
+            want = run()
+            assert torch.equal(got[0], want.detach()) and torch.equal(got[1], torch.autograd.grad(want, leaf, dy)[0]), (i, seed)
+            del want
