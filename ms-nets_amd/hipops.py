@@ -652,6 +652,98 @@ def clip_grads(grads, max_norm, out=None):
     return norm
 
 
+def _steps(t):
+    """[(bytes, steps)] from a tensor's first byte to any other: its dimensions of more than one entry, and the bytes of an element."""
+    size = t.element_size()
+    return [(s * size, n - 1) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, size - 1)]
+
+
+def _reaches(terms, target, budget=4096):
+    """Whether sum k * step = target for whole numbers low <= k <= high, terms = [(step, low, high)] with positive steps.  Longest step
+    first, where a k is tried only if the rest can still make up for it: two or three at a dimension whose steps pass what lies inside
+    it.  Where that leaves more to try than the budget, the answer is yes."""
+    merged = {}
+    for step, low, high in terms:
+        a, b = merged.get(step, (0, 0))
+        merged[step] = (a + low, b + high)
+    steps = sorted(merged, reverse=True)
+    rest = [(0, 0)]                                         # least and most that the steps behind each one add up to
+    for step in reversed(steps):
+        a, b = merged[step]
+        rest.append((rest[-1][0] + step * a, rest[-1][1] + step * b))
+    rest.reverse()
+    todo = [(0, target)]
+    while todo:
+        i, left = todo.pop()
+        if i == len(steps):
+            return True                                     # (rest[-1] lets nothing but left = 0 come this far)
+        step, (a, b), (least, most) = steps[i], merged[steps[i]], rest[i + 1]
+        for k in range(max(a, -((most - left) // step)), min(b, (left - least) // step) + 1):
+            budget -= 1
+            if budget < 0:
+                return True
+            todo.append((i + 1, left - k * step))
+    return False
+
+
+def _overlap(t, o):
+    """Whether a byte of memory belongs to both tensors, whatever their strides (where that is hard to say: yes)."""
+    (a, b), (c, d) = _extent(t), _extent(o)
+    if not t.numel() or not o.numel() or a >= d or c >= b:
+        return False
+    return _reaches([(s, 0, n) for s, n in _steps(t) if s] + [(s, -n, 0) for s, n in _steps(o) if s], c - a)
+
+
+def _overlaps_itself(t):
+    """Whether two places of a tensor share memory: some difference of two places, its first k > 0 in the order of the dimensions, is
+    less than an element away from nothing."""
+    if not t.numel():
+        return False
+    steps = _steps(t)
+    dims, inner = steps[:-1], steps[-1][1]
+    if any(s == 0 for s, _ in dims):
+        return True
+    return any(_reaches([(s, 1, n)] + [(s2, -n2, n2) for s2, n2 in dims[i + 1:]] + [(1, -inner, inner)], 0) for i, (s, n) in enumerate(dims))
+
+
+def _side_by_side(spans):
+    """Whether each of the tensors keeps to an arc of its own modulo their longest step: slices of one matrix's columns, 1000 of which
+    would be half a million pairs.  No: they may overlap."""
+    period = max(s for v in spans for s, _ in _steps(v[2]))
+    arcs = sorted((v[0] % period, 1 + sum(s * n for s, n in _steps(v[2]) if s != period)) for v in spans)
+    ends = [at + length for at, length in arcs]
+    return all(end <= at for end, (at, _) in zip(ends, arcs[1:])) and ends[-1] <= arcs[0][0] + period
+
+
+def _check_overlaps(grads, outs):
+    """Refuses outputs that share memory with each other or with a gradient other than their own: as the kernels' entry does, which
+    sees only the stand-ins of tensors that are laid out first."""
+    spans = []                                              # (first byte, behind the last, tensor, whether it is written)
+    for t, o in zip(grads, outs):
+        if not t.numel():
+            continue
+        spans.append((*_extent(o), o, True))
+        if t is not o and (t.data_ptr() != o.data_ptr() or t.dtype != o.dtype or t.stride() != o.stride()):
+            spans.append((*_extent(t), t, False))
+    spans.sort(key=lambda v: v[:2])
+    first = 0
+    while first < len(spans):
+        end, n = spans[first][1], 1                         # a run of tensors whose extents touch
+        while first + n < len(spans) and spans[first + n][0] < end:
+            end = max(end, spans[first + n][1])
+            n += 1
+        run = spans[first:first + n]
+        first += n
+        if n == 1 or _side_by_side(run):
+            continue
+        for i, v in enumerate(run):
+            for u in run[i + 1:]:
+                if u[0] >= v[1]:
+                    break
+                if (v[3] or u[3]) and _overlap(v[2], u[2]):
+                    raise RuntimeError("clip_grads: a tensor to be written overlaps another one of the call (is a gradient listed twice?)")
+
+
 def _clip_layout(grads, outs):
     """What clip_grads refuses, and contiguous stand-ins for tensors of other layouts: (inputs, outputs, [(tensor, stand-in that holds
     its new values)])."""
@@ -668,6 +760,8 @@ def _clip_layout(grads, outs):
             raise ValueError("a tensor to be written requires a gradient itself")
         if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
             raise ValueError("a tensor to be written is expanded: its values share memory")
+        if not _is_dense(o) and _overlaps_itself(o):
+            raise ValueError("a tensor to be written overlaps itself: its values share memory")
         _refuse_graph(t, "grads[%d]" % i)
         t, o = t.detach(), o.detach()
         if not t.is_neg() and not o.is_neg() and _is_dense(t) and (t.stride() == o.stride() or (t.is_contiguous() and o.is_contiguous())):
@@ -677,6 +771,7 @@ def _clip_layout(grads, outs):
             src.append(t.contiguous().resolve_neg().view(-1))
             dst.append(torch.empty(src[-1].shape, device=o.device, dtype=o.dtype))
             back.append((o, dst[-1].view(o.shape)))
+    _check_overlaps(grads, outs)
     return src, dst, back
 
 

@@ -246,3 +246,25 @@ def test_capture_beside_a_live_eager_graph_of_other_types_and_strides(gpu):
             want = run()
             assert torch.equal(got[0], want.detach()) and torch.equal(got[1], torch.autograd.grad(want, leaf, dy)[0]), (i, seed)
             del want
+
+
+# ---- lists of strided gradients ------------------------------------------------------------------------------------------------
+
+def test_strided_gradients_that_share_memory(gpu):
+    base = make((10, 12), F32, False)[0]
+    before = base.clone()
+    for bad in ([base[:, ::2], base[:, ::2]], [base, base[:, :3]], [base[:, 1:], base[:4, :1], base[3:, 2:3]]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            hipops.clip_grads(bad, 1.0)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            hipops.clip_grads([t.clone() for t in bad], 1.0, out=bad)
+        assert torch.equal(base, before)
+        assert abs(float(hipops.grad_norm(bad)) - sum(float(t.double().square().sum()) for t in bad) ** 0.5) <= 1e-5      # read only
+    shared = base.view(-1).as_strided((4, 3), (2, 1))
+    with pytest.raises(ValueError, match="overlaps itself"):
+        hipops.clip_grads([shared], 1.0)
+    assert torch.equal(base, before)
+    norm = hipops.clip_grads([base[:, ::2], base[:, 1:6:2], base[:, 7::2].t()], 1.0)          # beside each other: each value once
+    want = float(before.double().norm())
+    assert abs(float(norm) - want) <= 2 * U * want
+    within(base, (before.double() / (want + 1e-6), 4 * U * before.double().abs()), "values")

@@ -13,3 +13,102 @@ def test_graphs_are_refused_in_grad_mode_only():
     hipops._refuse_graph(p.detach(), "t")
     with torch.no_grad():
         hipops._refuse_graph(p, "t")
+
+
+def _bytes_of(t):
+    first = t.data_ptr()
+    at = torch.zeros((), dtype=torch.int64)
+    for s, n in zip(t.stride(), t.shape):
+        at = at[..., None] + torch.arange(n) * s
+    at = at.reshape(-1) * t.element_size() + first
+    return at, set((at[:, None] + torch.arange(t.element_size())).reshape(-1).tolist())
+
+
+def _random_view(base, rng):
+    """A view of base's memory, now and then one whose values share places."""
+    flat = base.view(torch.bfloat16) if rng.random() < 0.3 else base
+    dims = rng.randint(0, 4)
+    shape = [rng.randint(1, 4) for _ in range(dims)]
+    if rng.random() < 0.6:                     # nested, in any order: a slice of a dense tensor
+        at, stride = 1, [0] * dims
+        for i in rng.sample(range(dims), dims):
+            stride[i] = at * rng.choice([1, 1, 1, 2, 3])
+            at = stride[i] * (shape[i] + rng.randint(0, 1))
+    else:
+        stride = [rng.randint(0, 12) for _ in range(dims)]
+    reach = sum((n - 1) * s for n, s in zip(shape, stride))
+    if reach >= flat.numel():
+        return flat[:5]
+    return flat.as_strided(shape, stride, rng.randint(0, min(flat.numel() - reach - 1, 60)))
+
+
+def test_overlaps_of_any_strides():
+    """Against the places listed one by one."""
+    import random
+    rng, base, seen = random.Random(0), torch.zeros(4000), [0, 0, 0]
+    for _ in range(3000):
+        a, b = _random_view(base, rng), _random_view(base, rng)
+        (pa, sa), (_, sb) = _bytes_of(a), _bytes_of(b)
+        assert hipops._overlap(a, b) == hipops._overlap(b, a) == bool(sa & sb), (a.shape, a.stride(), b.shape, b.stride())
+        own = len(sa) < a.numel() * a.element_size()
+        assert hipops._overlaps_itself(a) == own, (a.shape, a.stride())
+        seen[0] += bool(sa & sb)
+        seen[1] += not sa & sb and a.data_ptr() < b.data_ptr() < a.data_ptr() + max(sa) - min(sa)
+        seen[2] += own
+    assert min(seen) > 100, seen
+    assert not hipops._overlap(base[:0], base) and not hipops._overlaps_itself(base[:0])
+    # hard to say within the budget: taken for an overlap
+    wide = torch.empty(1, dtype=torch.float32).as_strided((1,), (1,))
+    assert hipops._reaches([(2 ** 20 + 2 * k, 0, 2 ** 12) for k in range(12)], 2 ** 33 + 1) and wide.numel() == 1
+
+
+def test_overlaps_in_lists():
+    """Three outputs and three gradients in the same memory, some in place: refused if a written place belongs to anything else."""
+    import random
+    rng, base, refused = random.Random(1), torch.zeros(4000), 0
+    for _ in range(3000):
+        outs = [_random_view(base, rng) for _ in range(3)]
+        grads = [o if rng.random() < 0.7 else _random_view(base[500 * rng.randint(0, 1):], rng) for o in outs]
+        places = [_bytes_of(t)[1] for t in outs + grads]
+        want = any(places[i] & places[j] for i in range(3) for j in range(i + 1, 6)
+                   if not (j == i + 3 and (outs[i] is grads[i] or (outs[i].data_ptr() == grads[i].data_ptr() and outs[i].dtype == grads[i].dtype
+                                                                   and outs[i].stride() == grads[i].stride()))))
+        try:
+            hipops._check_overlaps(grads, outs)
+            assert not want
+        except RuntimeError:
+            assert want
+            refused += 1
+    assert 500 < refused < 2900, refused
+
+
+def test_clipping_refuses_overlaps_of_any_strides(monkeypatch):
+    monkeypatch.setattr(hipops, "_require_gpu", lambda t, name: t)          # (the layout is host code: any tensors will do)
+    base, spare = torch.zeros(10, 12), [torch.zeros(10, 6), torch.zeros(10, 6)]
+    even, odd, left = base[:, ::2], base[:, 1::2], base[:, :3]
+    for bad in ([even, even], [base, left], [left, base], [even, base[:, 2:4]], [base[:, :6].t(), base[3:4, 5:7]], [even[2], base[:, 4]]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            hipops._clip_layout(bad, bad)
+        hipops._clip_layout(bad, [torch.zeros_like(t) for t in bad])          # read only
+    for src, dst in ((spare, [even, even]), (spare, [base[:, :6], base[:, 5:11]]), ([even, spare[0]], [spare[1], even]), ([base[:, 1:7]], [base[:, :6]]),
+                     ([even.bfloat16(), base[:, 6:]], [even, spare[0]])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            hipops._clip_layout(src, dst)
+    for shared in (torch.zeros(40).as_strided((4, 3), (2, 1)), torch.zeros(40).as_strided((3, 4, 2), (4, 2, 3))):
+        with pytest.raises(ValueError, match="overlaps itself"):
+            hipops._clip_layout([shared], [shared])
+        hipops._clip_layout([shared], [torch.zeros(shared.shape)])
+    for good in ([even, odd], [base[:, :6], base[:, 6:]], [base[:, 3 * i:3 * i + 3].t() for i in range(4)], [even[:, None], odd[3:]], [base[:5], base.t()[:, 5:]]):
+        src, dst, back = hipops._clip_layout(good, good)
+        assert len(src) == len(dst) == len(good)
+    wide = torch.zeros(64, 4000)
+    columns = [wide[:, i:i + 8] for i in range(0, 4000, 8)]                    # many slices of one matrix
+    assert len(hipops._clip_layout(columns, columns)[2]) == 500
+    for one in (wide[7:9, 100:101], wide[:, 3992:], wide.t()[3999:]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            hipops._clip_layout(columns + [one], columns + [one])
+    around = [wide[1:40, :7], wide[:39, 4:4000:4000], wide.view(-1)[4000 * 50:4000 * 50 + 6]]
+    around += [torch.as_strided(wide, (38, 8), (4000, 1), 3996)]                # rows that go over a row's end
+    with pytest.raises(RuntimeError, match="overlaps"):
+        hipops._clip_layout(around, around)
+    assert hipops._overlap(around[0], around[3]) and not hipops._overlap(around[1], around[2])
