@@ -239,7 +239,8 @@ int msnet_conv3d_k3_cout1(const float* x, const float* w, float wscale, const fl
  *   y = act( (x - mean) / sqrt(var + eps) * weight[c] + bias[c] (+ residual) ),   mean and var over the S rows and C/G channels
  * of one sample and group.  x, residual, y: [N][S][C] of `dtype` (0 float32, 1 float16, 2 bfloat16), S = D*H*W; channels are
  * consecutive, rows (_ss) and samples (_sn) lie that many elements apart (a channel slice of a wider tensor, 0 for a broadcast
- * input).  y may be x or residual itself (same strides), and must not overlap them otherwise.  act: 0 none, 1 ReLU, 2 SiLU.
+ * input).  y may be x or residual itself (same strides), and must not overlap them otherwise, nor weight, bias or stats.
+ * act: 0 none, 1 ReLU, 2 SiLU.
  * weight, bias: f32[C] or NULL (1 and 0).  stats: double[N][G][2], gets mean and 1 / sqrt(var + eps) for the backward; or NULL.
  * Sums are 64-bit, in a fixed order.  float32 outputs raise bit 0 of the calling thread's overflow word as the convs' do.
  * workspace: msnet_group_norm_workspace_bytes() bytes, 16-byte aligned (0: not needed).  N or S zero: nothing is done. */

@@ -506,6 +506,14 @@ def _check_out(out, t, name):
     raise ValueError("out overlaps %s: pass %s itself, or memory of its own" % (name, name))
 
 
+def _check_out_params(out, *params):
+    """out may share no memory with weight or bias, which every workgroup reads while others write."""
+    a, b = _extent(out)
+    for p in params:
+        if p is not None and p.data_ptr() < b and p.data_ptr() + p.numel() * p.element_size() > a and _overlap(out, p):
+            raise ValueError("out overlaps weight or bias: pass memory of its own")
+
+
 def _check_norm_args(x, groups, weight, bias, eps, act, residual):
     _require_gpu(x, "x")
     if x.dim() < 2:
@@ -574,6 +582,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", residual
             raise ValueError("out must not be a negated view")
         _check_out(out, x, "x")
         _check_out(out, residual, "residual")
+        _check_out_params(out, weight, bias)
     lib, code, xs, ys, rs = _lib.load(), _DTYPE_CODES[x.dtype], _row_strides(x), _row_strides(out), _row_strides(residual) if residual is not None else (0, 0)
     nbytes = lib.msnet_group_norm_workspace_bytes(code, n, s, c, groups)
     ws = None if not nbytes else _new(((nbytes + 3) // 4,), x.device) if _tls.arena is not None else torch.empty(nbytes, device=x.device, dtype=torch.uint8)

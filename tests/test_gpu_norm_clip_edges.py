@@ -268,3 +268,21 @@ def test_strided_gradients_that_share_memory(gpu):
     want = float(before.double().norm())
     assert abs(float(norm) - want) <= 2 * U * want
     within(base, (before.double() / (want + 1e-6), 4 * U * before.double().abs()), "values")
+
+
+# ---- out= ---------------------------------------------------------------------------------------------------------------------
+
+def test_out_over_the_parameters_is_refused(gpu):
+    x, w, b, _, _ = make((2, 20, 16), F32, False)
+    pool = torch.zeros(2 * 20 * 16 + 16, device="cuda")
+    out, beside = pool[:640].view(2, 20, 16), pool[640:]
+    for shared in (pool[:16], pool[630:646]):
+        for kw in (dict(weight=shared, bias=b), dict(weight=w, bias=shared)):
+            with pytest.raises(ValueError, match="weight or bias"):
+                hipops.group_norm(x, 4, out=out, **kw)
+    assert not pool.any()
+    beside.copy_(b)
+    assert torch.equal(hipops.group_norm(x, 4, w, beside, out=out), hipops.group_norm(x, 4, w, b))
+    cast = pool[:8].view(F16)                  # of another type: read, as a copy, before anything is written
+    want = hipops.group_norm(x, 4, cast.clone(), b)
+    assert torch.equal(hipops.group_norm(x, 4, cast, b, out=out), want)

@@ -112,3 +112,17 @@ def test_clipping_refuses_overlaps_of_any_strides(monkeypatch):
     with pytest.raises(RuntimeError, match="overlaps"):
         hipops._clip_layout(around, around)
     assert hipops._overlap(around[0], around[3]) and not hipops._overlap(around[1], around[2])
+
+
+def test_out_over_the_parameters():
+    base = torch.zeros(1000)
+    out = base[:960].view(2, 20, 24)[..., :8]
+    check = hipops._check_out_params
+    check(out, None, None)
+    check(out, torch.zeros(8), base[960:968])
+    check(out, base[8:16], base[24 * 5 + 16:24 * 6])                            # between its rows
+    check(out[:0], base[:8])
+    for bad in (base[:8], base[4:12], base[17:25], base[24 * 39:24 * 39 + 8], base.view(torch.bfloat16)[14:22]):
+        for params in ((bad, None), (None, bad), (torch.zeros(8), bad)):
+            with pytest.raises(ValueError, match="weight or bias"):
+                check(out, *params)
