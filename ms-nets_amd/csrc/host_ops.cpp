@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <cmath>
 #include <vector>
 
 #include "../../include/msnet_hip.h"
@@ -201,7 +202,7 @@ PyObject* group_norm(PyObject*, PyObject* args) {
         for (const Tensor* t : {&x, &w, &b, &r}) refuse_tangent(*t, "group_norm");
     const auto device = c10::hip::current_device();
     Rows any;
-    if (!ordinary(x, device) || x.dim() < 2 || !rows_of(x, &any) || x.size(-1) < 1 || groups < 1 || x.size(-1) % groups || !(eps >= 0.) || eps > 1e300 ||
+    if (!ordinary(x, device) || x.dim() < 2 || !rows_of(x, &any) || x.size(-1) < 1 || groups < 1 || x.size(-1) % groups || !(eps >= 0. && std::isfinite(eps)) ||
         x.size(0) > INT32_MAX || x.size(-1) > INT32_MAX)
         Py_RETURN_NONE;
     for (const Tensor* p : {&w, &b})

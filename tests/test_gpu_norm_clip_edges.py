@@ -286,3 +286,19 @@ def test_out_over_the_parameters_is_refused(gpu):
     cast = pool[:8].view(F16)                  # of another type: read, as a copy, before anything is written
     want = hipops.group_norm(x, 4, cast.clone(), b)
     assert torch.equal(hipops.group_norm(x, 4, cast, b, out=out), want)
+
+
+@pytest.mark.parametrize("eps", [0.0, 5e-324, 1e30, 1e300, 1e305, 1.7e308])
+@pytest.mark.parametrize("shape", BOTH_WAYS)
+def test_any_finite_eps(gpu, shape, eps):
+    x, w, b, r, dy = make(shape, F32, True)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = hipops.group_norm(x, 4, w, b, eps=eps, act="relu", residual=r)
+    grads = torch.autograd.grad(y, leaves, dy)
+    want = norm64(x.detach(), 4, w.detach(), b.detach(), eps, "relu", r.detach(), dy)
+    within(y.detach(), want["y"], "y")
+    for k, v in zip(("dx", "dweight", "dbias", "dresidual"), grads):
+        if k == "dweight":                     # beyond eps = 1e76, 1 / sqrt(eps) and xhat are below float32's normal numbers
+            value, allowed = want[k]
+            want[k] = value, allowed + 2.0 ** -149 * float(dy.abs().sum())
+        within(v, want[k], k)
