@@ -241,12 +241,13 @@ PyObject* clip(PyObject*, PyObject* args) {
         if (!THPVariable_Check(PyList_GET_ITEM(list, i))) Py_RETURN_NONE;
         const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
         if (tangents) refuse_tangent(t, write ? "clip_grads" : "grad_norm");
-        if (!ordinary(t, device) || !t.is_contiguous() || (grad && t.requires_grad())) Py_RETURN_NONE;
+        if (!ordinary(t, device) || !t.is_contiguous()) Py_RETURN_NONE;
+        PyObject* po = write ? PyList_GET_ITEM(outs, i) : nullptr;
+        if (grad && po != PyList_GET_ITEM(list, i) && t.requires_grad()) Py_RETURN_NONE;       // (in place: asked of the output, below)
         in[i] = t.const_data_ptr();
         lengths[i] = t.numel();
         types[i] = (uint8_t)type_code(t.scalar_type());
         if (!write) continue;
-        PyObject* po = PyList_GET_ITEM(outs, i);
         if (!THPVariable_Check(po)) Py_RETURN_NONE;
         const Tensor& o = THPVariable_Unpack(po);
         if (tangents) refuse_tangent(o, "clip_grads");
