@@ -142,6 +142,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &residual = saved[3], &stats = saved[4];
         const int64_t groups = ctx->saved_data["groups"].toInt(), act = ctx->saved_data["act"].toInt();
         torch::autograd::variable_list out(7);
+        if (tangents_exist()) refuse_tangent(grads[0], "the gradient of group_norm");
         {
             c10::AutoGradMode off(false);
             Tensor dy = grads[0].resolve_neg();            // (a view with its sign bit to be applied is none the kernels can read)

@@ -302,3 +302,16 @@ def test_any_finite_eps(gpu, shape, eps):
             value, allowed = want[k]
             want[k] = value, allowed + 2.0 ** -149 * float(dy.abs().sum())
         within(v, want[k], k)
+
+
+def test_forward_over_reverse_is_refused(gpu):
+    """A tangent of the incoming gradient would be lost in the backward as one of x is in the forward."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w, b, r, dy = make((2, 60, 16), F32, True)
+    for act, res in (("relu", None), ("silu", r.clone().requires_grad_()), ("none", r.clone().requires_grad_())):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)] + ([res] if res is not None else [])
+        y = hipops.group_norm(leaves[0], 4, leaves[1], leaves[2], act=act, residual=res)
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaves, forward_ad.make_dual(dy, torch.ones_like(dy)), retain_graph=True)
+            torch.autograd.grad(y, leaves, dy)
