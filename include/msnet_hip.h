@@ -243,15 +243,16 @@ int msnet_conv3d_k3_cout1(const float* x, const float* w, float wscale, const fl
  * act: 0 none, 1 ReLU, 2 SiLU.
  * weight, bias: f32[C] or NULL (1 and 0).  stats: double[N][G][2], gets mean and 1 / sqrt(var + eps) for the backward; or NULL.
  * Sums are 64-bit, in a fixed order.  float32 outputs raise bit 0 of the calling thread's overflow word as the convs' do.
- * workspace: msnet_group_norm_workspace_bytes() bytes, 16-byte aligned (0: not needed).  N or S zero: nothing is done. */
+ * workspace: msnet_group_norm_workspace_bytes() bytes, 16-byte aligned (0: not needed).  N or S zero: nothing is done.  Refused:
+ * more samples and channel chunks than a launch of 2^32 threads takes (about 16 million short samples). */
 size_t msnet_group_norm_workspace_bytes(int dtype, int N, long S, int C, int G);
 int    msnet_group_norm(const void* x, const float* weight, const float* bias, const void* residual, void* y, double* stats,
                         int dtype, int act, int N, long S, int C, int G, double eps, long x_sn, long x_ss, long r_sn, long r_ss,
                         long y_sn, long y_ss, void* workspace, size_t workspace_bytes, msnet_stream_t stream);
 /* Its gradients from dy and what the forward had (stats included).  dx, dresidual: dense [N][S][C]; dweight, dbias: f32[C]; each
- * may be NULL.  dresidual only with an activation (without one it is dy itself).  The derivative of the ReLU is 0 at 0 and 1 at a
- * NaN, which the forward passes on too; on which side of 0 a value lies is decided in 64 bits.  N or S zero: dweight and dbias
- * become zero. */
+ * memory of its own, or NULL.  dresidual only with an activation (without one it is dy itself).  The derivative of the ReLU is 0 at
+ * 0 and 1 at a NaN, which the forward passes on too; on which side of 0 a value lies is decided in 64 bits.  N or S zero: dweight
+ * and dbias become zero.  The workspace holds 16 bytes a sample and channel where N > 1 and samples are short. */
 size_t msnet_group_norm_backward_workspace_bytes(int dtype, int N, long S, int C, int G);
 int    msnet_group_norm_backward(const void* dy, const void* x, const float* weight, const float* bias, const void* residual,
                                  const double* stats, void* dx, void* dresidual, float* dweight, float* dbias, int dtype, int act,

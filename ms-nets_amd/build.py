@@ -43,7 +43,7 @@ SOURCES = [
 ]
 COMMON = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-Wall", "-Wno-unused-function",
           "-fno-gpu-rdc",
-          # gfx950's packed float instructions (v_pk_add_f32 and its kin) have given wrong results now and then; hipcc forms them by itself
+          # without gfx950's packed float instructions (v_pk_add_f32 and its kin), which hipcc forms by itself: they are avoided throughout
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

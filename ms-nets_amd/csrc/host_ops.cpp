@@ -1,5 +1,5 @@
 // Python module _host: the group norm and gradient clipping as torch operators over the C ABI (include/msnet_hip.h), the group norm
-// with its gradient.  Both work on calls of a few microseconds: reading a list's tensors from Python costs 0.6 us each (here 0.02),
+// with its gradient.  Both work on calls of a few microseconds: reading a list's tensors from Python costs 0.6 us each (here 0.05),
 // and a gradient written in Python another 25 us and the interpreter's lock on the autograd thread.  Only this file knows torch's
 // C++ interface; libmsnet_hip.so does not, its entry points are handed over by address (bind).
 //

@@ -105,7 +105,8 @@ def get_epe_rate_gpu(disp, prediction, max_disp=192, threshold=3.0):
 def clip_grad_norm_(parameters, max_norm):
     """torch.nn.utils.clip_grad_norm_ for a training loop around these kernels: scales the gradients of `parameters` (an iterable, or
     one tensor; those without a gradient are skipped) in place to a global 2-norm of at most max_norm and returns the norm before
-    as a float32 scalar on the device.  Two launches for the whole model, and no host synchronisation (hipops.clip_grads)."""
+    as a float32 scalar on the device.  Two launches for up to 176 gradients, one more for every 216 of a longer list, and no host
+    synchronisation (hipops.clip_grads)."""
     import torch
     from . import hipops
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
