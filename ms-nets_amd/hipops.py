@@ -733,7 +733,7 @@ def _check_overlaps(grads, outs):
         if not t.numel():
             continue
         spans.append((*_extent(o), o, True))
-        if t is not o and (t.data_ptr() != o.data_ptr() or t.dtype != o.dtype or t.stride() != o.stride()):
+        if t is not o and (t.data_ptr() != o.data_ptr() or t.dtype != o.dtype or _steps(t) != _steps(o)):
             spans.append((*_extent(t), t, False))
     spans.sort(key=lambda v: v[:2])
     first = 0
