@@ -39,9 +39,12 @@ void succeed(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed: ",
 
 int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1; }
 
-bool ordinary(const Tensor& t, c10::DeviceIndex device) {
-    return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && type_code(t.scalar_type()) >= 0 && !t.is_neg();
+// The type's code, or -1: not an ordinary tensor of the device.
+int ordinary_code(const Tensor& t, c10::DeviceIndex device) {
+    return t.defined() && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() ? type_code(t.scalar_type()) : -1;
 }
+
+bool ordinary(const Tensor& t, c10::DeviceIndex device) { return ordinary_code(t, device) >= 0; }
 
 // Forward-mode tangents are not carried on: a result without one would stand for a derivative of zero.  A call asks once whether any
 // can exist (asking 1000 views and their outputs one by one took 45 us).
@@ -238,25 +241,35 @@ PyObject* clip(PyObject*, PyObject* args) {
     std::vector<void*> out(write ? n : 0);
     std::vector<int64_t> lengths(n);
     std::vector<uint8_t> types(n), out_types(write ? n : 0);
+    std::vector<at::TensorImpl*> written;                  // (the caller's list holds them, and the interpreter's lock is not given up)
+    written.reserve(write ? n : 0);
     for (Py_ssize_t i = 0; i < n; ++i) {
         if (!THPVariable_Check(PyList_GET_ITEM(list, i))) Py_RETURN_NONE;
         const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
         if (tangents) refuse_tangent(t, write ? "clip_grads" : "grad_norm");
-        if (!ordinary(t, device) || !t.is_contiguous()) Py_RETURN_NONE;
+        const int code = ordinary_code(t, device);
+        if (code < 0 || !t.is_contiguous()) Py_RETURN_NONE;
         PyObject* po = write ? PyList_GET_ITEM(outs, i) : nullptr;
-        if (grad && po != PyList_GET_ITEM(list, i) && t.requires_grad()) Py_RETURN_NONE;       // (in place: asked of the output, below)
+        if (grad && t.requires_grad()) Py_RETURN_NONE;
         in[i] = t.const_data_ptr();
         lengths[i] = t.numel();
-        types[i] = (uint8_t)type_code(t.scalar_type());
+        types[i] = (uint8_t)code;
         if (!write) continue;
+        if (po == PyList_GET_ITEM(list, i)) {              // in place
+            out[i] = t.mutable_data_ptr();
+            out_types[i] = (uint8_t)code;
+            written.push_back(t.unsafeGetTensorImpl());
+            continue;
+        }
         if (!THPVariable_Check(po)) Py_RETURN_NONE;
         const Tensor& o = THPVariable_Unpack(po);
         if (tangents) refuse_tangent(o, "clip_grads");
-        if (!ordinary(o, device) || !o.is_contiguous() || (o.scalar_type() != t.scalar_type() && o.scalar_type() != at::kFloat) ||
-            (!o.is_same(t) && o.sizes() != t.sizes()) || (grad && o.requires_grad()))
+        const int out_code = ordinary_code(o, device);
+        if (out_code < 0 || !o.is_contiguous() || (out_code != code && out_code != 0) || o.sizes() != t.sizes() || (grad && o.requires_grad()))
             Py_RETURN_NONE;
         out[i] = o.mutable_data_ptr();
-        out_types[i] = (uint8_t)type_code(o.scalar_type());
+        out_types[i] = (uint8_t)out_code;
+        written.push_back(o.unsafeGetTensorImpl());
     }
     const auto options = at::TensorOptions().device(at::kCUDA, device);
     Tensor norm = at::empty({}, options.dtype(at::kFloat));
@@ -265,10 +278,8 @@ PyObject* clip(PyObject*, PyObject* args) {
     succeed(clip_grads(in.data(), write ? out.data() : nullptr, lengths.data(), types.data(), write ? out_types.data() : nullptr, (int)n, max_norm,
                        data<float>(norm), data(ws), bytes, stream_of(device)),
             "msnet_clip_grads");
-    for (Py_ssize_t i = 0; write && i < n; ++i) {          // written behind autograd's back: what saved them finds out
-        const Tensor& o = THPVariable_Unpack(PyList_GET_ITEM(outs, i));
-        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
-    }
+    for (const auto& o : written)                          // behind autograd's back: what saved them finds out
+        if (!o->is_inference()) o->bump_version();
     return THPVariable_Wrap(norm);
     END_HANDLE_TH_ERRORS
 }

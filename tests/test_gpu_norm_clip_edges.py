@@ -315,3 +315,53 @@ def test_forward_over_reverse_is_refused(gpu):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, leaves, forward_ad.make_dual(dy, torch.ones_like(dy)), retain_graph=True)
             torch.autograd.grad(y, leaves, dy)
+
+
+def test_lists_in_one_buffer_are_taken_or_refused(gpu):
+    """Contiguous tensors in one buffer, in order and out of it, empty ones among them, in place and not: refused if and only if a
+    written byte belongs to another tensor of the call, and right where they are taken."""
+    import random
+    rng, seen = random.Random(3), [0, 0]
+    start = make((4096,), F32, False)[0]
+    for trial in range(2000):
+        buffer, k = start.clone(), rng.randint(1, 6)
+
+        def views(types):
+            at, out = rng.choice([0, 0, 16, 64]), []
+            for t in types:
+                flat, n = buffer.view(t), rng.choice([0, 1, 2, 3, 5, 8, 40])
+                out.append(flat[at * 4 // t.itemsize:][:n])
+                at += -(-n * t.itemsize // 4) + rng.choice([0, 0, 1, 3, 16])
+            return out
+        types = [rng.choice([F32, F32, F16, BF16]) for _ in range(k)]
+        outs = views(types)
+        grads = [o if rng.random() < 0.6 else start.to(o.dtype if o.dtype != F32 else rng.choice([F32, F16, BF16]))[rng.randint(0, 99):][:o.numel()]
+                 for o in outs]
+        if rng.random() < 0.3:
+            i = rng.randrange(k)
+            grads[i] = buffer.view(outs[i].dtype)[rng.randint(0, 200):][:outs[i].numel()]
+        both = list(zip(grads, outs))
+        if rng.random() < 0.3:
+            rng.shuffle(both)
+        grads, outs = [t for t, _ in both], [o for _, o in both]
+        try:
+            hipops._check_overlaps(grads, outs)
+            refused = False
+        except RuntimeError:
+            refused = True
+        seen[refused] += 1
+        before = [t.double() for t in grads]
+        if refused:
+            with pytest.raises(RuntimeError, match="overlaps"):
+                hipops.clip_grads(grads, 0.5, out=outs)
+            assert torch.equal(buffer.view(torch.int32), start.view(torch.int32))
+            continue
+        if any(not bool(torch.isfinite(t).all()) for t in before):               # (16-bit views of floats)
+            continue
+        norm = sum(float(t.square().sum()) for t in before) ** 0.5
+        got = hipops.clip_grads(grads, 0.5, out=outs)
+        assert abs(float(got) - norm) <= 2 * U * norm
+        for t, o in zip(before, outs):
+            want = t * min(1.0, 0.5 / (norm + 1e-6))
+            within(o, (want, (3 * U + torch.finfo(o.dtype).eps / 2) * want.abs() + torch.finfo(o.dtype).smallest_normal * torch.finfo(o.dtype).eps), "values")
+    assert min(seen) > 100, seen

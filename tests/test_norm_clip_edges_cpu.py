@@ -136,3 +136,42 @@ def test_the_same_memory_with_other_strides_of_single_entries(monkeypatch):
     assert len(hipops._clip_layout([t, other], [o, other])[0]) == 2
     with pytest.raises(RuntimeError, match="overlaps"):
         hipops._clip_layout([t, other], [base[1:6].view(1, 5), other])
+
+
+def test_c_entry_overlaps(hiplib):
+    """Lists of contiguous tensors, in order and out of it, empty ones among them: refused where a written byte belongs to another
+    tensor of the call.  (Lists that are taken are launched: those are compared on the GPU.)"""
+    import ctypes
+    import random
+    rng, seen = random.Random(2), [0, 0]
+    size = {0: 4, 1: 2, 2: 2}
+
+    def call(src, dst, n, st, dt, ws):
+        k = len(n)
+        return hiplib.msnet_clip_grads((ctypes.c_uint64 * k)(*src), (ctypes.c_uint64 * k)(*dst), (ctypes.c_int64 * k)(*n), bytes(st), bytes(dt), k, 1.0,
+                                       ctypes.c_void_p(1 << 20), ws, 1 << 16, None)
+    for trial in range(4000):
+        k = rng.randint(1, 5)
+        n = [rng.choice([0, 1, 2, 3, 5, 8]) for _ in range(k)]
+        dt = [rng.choice([0, 0, 1, 2]) for _ in range(k)]
+        st = [rng.choice([1, 2, 0]) if d == 0 else d for d in dt]
+        place = lambda at, t: [at.append(at[-1] + n[i] * size[t[i]] + 4 * rng.choice([0, 0, 1, 3])) or at[-2] for i in range(k)]      # noqa: E731
+        dst, src = place([4096], dt), place([rng.choice([4096, 4100, 4160, 8192, 16384])], st)
+        for t in (dst, src):
+            if rng.random() < 0.3:
+                rng.shuffle(t)
+        for i in range(k):
+            if rng.random() < 0.4 and st[i] == dt[i]:
+                src[i] = dst[i]
+        if rng.random() < 0.2:
+            dst[rng.randrange(k)] += rng.choice([-4, 4])
+        out = [set(range(dst[i], dst[i] + n[i] * size[dt[i]])) for i in range(k)]
+        read = [set(range(src[i], src[i] + n[i] * size[st[i]])) for i in range(k)]
+        want = any(out[i] & out[j] for i in range(k) for j in range(i)) or any(
+            out[i] & read[j] for i in range(k) for j in range(k) if not (src[j] == dst[j] and st[j] == dt[j] and i == j))
+        if not want:
+            seen[0] += 1
+            continue
+        assert call(src, dst, n, st, dt, ctypes.c_void_p(1 << 20)) != 0 and b"overlaps" in hiplib.msnet_last_error(), (src, dst, n, st, dt)
+        seen[1] += 1
+    assert min(seen) > 1000, seen
